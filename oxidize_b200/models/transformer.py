@@ -16,7 +16,7 @@ GEMM kernel on the GPU path), the lm_head is vocabulary-parallel.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 from typing import List, Optional, Tuple
 
 import torch
@@ -338,7 +338,7 @@ class Transformer:
                             rows = 2 * cfg.gdn_k_heads * cfg.gdn_k_dim + cfg.gdn_v_heads * cfg.gdn_v_dim
                             c_shape, s_shape = (rows, max(1, cfg.gdn_conv - 1)), (cfg.gdn_v_heads, cfg.gdn_k_dim, cfg.gdn_v_dim)
                         else:
-                            c_shape, s_shape = (cfg.ssm_d_inner, max(1, cfg.ssm_d_conv - 1)), (cfg.ssm_d_inner, cfg.ssm_d_state)
+                            c_shape, s_shape = (cfg.ssm_d_conv, cfg.ssm_d_inner), (cfg.ssm_d_inner, cfg.ssm_d_state)
                         add_c = torch.zeros(16, L, *c_shape, dtype=torch.float32, device=self.device)
                         add_s = torch.zeros(16, L, *s_shape, dtype=torch.float32, device=self.device)
                         self._ssm_conv = add_c if self._ssm_conv is None else torch.cat([self._ssm_conv, add_c])
@@ -357,42 +357,32 @@ class Transformer:
         for key in [k for k in self._ssm_slots if k[0] == id(kv)]:
             del self._ssm_slots[key]
 
+    def _ssm_step(self, meta: BatchMeta, kv, first_layer: bool) -> BatchMeta:
+        """The step with its sequences' state slots, which the first layer with a state finds for all of them."""
+        if not first_layer:
+            return meta.extra["ssm_step"]
+        self._ssm_clock += 1
+        qs, first, pos0 = meta.query_start.tolist(), meta.block_tables[:, 0].tolist(), meta.positions.tolist()
+        slots = [self._ssm_slot(kv, first[b], pos0[qs[b]]) if qs[b + 1] > qs[b] else -1 for b in range(len(qs) - 1)]
+        step = replace(meta, state_slots=torch.tensor(slots, dtype=torch.int32, device=self.device))
+        meta.extra["ssm_step"] = step
+        return step
+
     def _mamba(self, lw: LayerWeights, layer: int, x: torch.Tensor, meta: BatchMeta, kv) -> torch.Tensor:
-        """Selective state-space mixer, sequence by sequence and token by token (the recurrence is sequential):
-        (u, z) = in_proj(x); u = silu(conv(u)); (dt, B, C) = x_proj(u); dt = softplus(dt_proj(dt) + b);
-        h = exp(A dt) h + dt B u; y = (h C + D u) silu(z); out_proj(y)."""
+        """Selective state-space mixer: (u, z) = in_proj(x); u = silu(conv(u)); (dt, B, C) = x_proj(u);
+        dt = softplus(dt_proj(dt) + b); h = exp(A dt) h + dt B u; y = (h C + D u) silu(z); out_proj(y)."""
         cfg, m = self.cfg, lw.ssm
-        di, N, K, R = cfg.ssm_d_inner, cfg.ssm_d_state, cfg.ssm_d_conv, cfg.ssm_dt_rank
-        xz = ops.linear(x, m.in_proj).float()
-        u_all, z_all = xz[:, :di], xz[:, di:]
-        qs, first = meta.query_start.tolist(), meta.block_tables[:, 0].tolist()
-        pos0 = meta.positions.tolist()
-        w, A, D = m.conv_kernel.float(), m.a.float(), m.d.float()
-        y = torch.empty_like(u_all)
-        if layer == 0:
-            self._ssm_clock += 1
-        for b in range(len(qs) - 1):
-            t0, t1 = qs[b], qs[b + 1]
-            if t1 == t0:
-                continue
-            slot = self._ssm_slot(kv, first[b], pos0[t0] if layer == 0 else -1)
-            win = torch.cat([self._ssm_conv[slot, layer], u_all[t0:t1].t()], dim=1)  # [di, K-1 + n]
-            conv = sum(w[:, j : j + 1] * win[:, j : j + (t1 - t0)] for j in range(K))
-            if m.conv_bias is not None:
-                conv = conv + m.conv_bias.float()[:, None]
-            uc = torch.nn.functional.silu(conv).t().contiguous()  # [n, di]
-            self._ssm_conv[slot, layer] = win[:, -(K - 1):] if K > 1 else win[:, :0]
-            # step size, B and C steer an exponential recurrence: these two narrow projections stay in float32 (plain
-            # products on the decoded matrices) instead of going through the bf16 GEMM
-            par = uc @ m.x_proj.dense_cache().float().t()
-            dt = torch.nn.functional.softplus(par[:, :R] @ m.dt_proj.dense_cache().float().t() + m.dt_bias.float())
-            Bm, Cm = par[:, R : R + N], par[:, R + N :]
-            h = self._ssm_state[slot, layer]
-            for i in range(t1 - t0):
-                h = torch.exp(A * dt[i][:, None]) * h + (dt[i] * uc[i])[:, None] * Bm[i][None, :]
-                y[t0 + i] = h @ Cm[i] + D * uc[i]
-            self._ssm_state[slot, layer] = h
-        return ops.linear((y * torch.nn.functional.silu(z_all)).to(x.dtype), m.out_proj)
+        di, N, R = cfg.ssm_d_inner, cfg.ssm_d_state, cfg.ssm_dt_rank
+        xz = ops.linear(x, m.in_proj)
+        step = self._ssm_step(meta, kv, layer == 0)
+        u = ops.causal_conv(xz[:, :di], m.conv_kernel, m.conv_bias, step, self._ssm_conv[:, layer])
+        # step size, B and C steer an exponential recurrence: these two narrow projections stay in float32 (plain
+        # products on the decoded matrices) instead of going through the bf16 GEMM
+        par = u @ m.x_proj.dense_cache().float().t()
+        dt = par[:, :R] @ m.dt_proj.dense_cache().float().t()
+        y = ops.selective_scan(u, dt, m.a, par[:, R : R + N], par[:, R + N :], m.d, xz[:, di:], m.dt_bias, step,
+                               self._ssm_state[:, layer], act_dtype=x.dtype)
+        return ops.linear(y, m.out_proj)
 
     def _gated_delta(self, lw: LayerWeights, layer: int, x: torch.Tensor, meta: BatchMeta, kv) -> torch.Tensor:
         """Gated delta rule (Qwen3.5's linear attention), sequence by sequence and token by token:

@@ -46,6 +46,12 @@ def _cuda_wkv():
     return _c
 
 
+def _cuda_ssm():
+    from . import cuda_ssm as _c
+
+    return _c
+
+
 class DepthStreams:
     """The embedding and the layers' results of a step, kept for the weighted sums that go on from layer to layer."""
 
@@ -222,6 +228,61 @@ def listed_mixer(x, lw, spec, ropes, meta, kv, kv_layer, state_layer, eps, carry
         o = ref.delta_rule(zr, lw.delta, d, meta, kv.states.data[state_layer], kv.states.windows[state_layer], eps)
         outs.append((o * sr).to(x.dtype))
     return tuple(outs) if lw.out_norms is not None else torch.cat(outs, dim=-1)
+
+
+@instrument("causal_conv")
+def causal_conv(x, w, bias, meta, window, act="silu", act_dtype=torch.float32, out=None):
+    """Short depthwise convolution of a step's rows, each sequence over its own: y[t, c] = act(sum_i w[c, i] x[t - (taps - 1) + i, c]
+    + bias[c]) in ``act_dtype``.  x [T, C] (bfloat16 or float32, possibly columns of a wider projection), w [C, taps] and bias [C]
+    float32, ``act`` "silu" or "none".  ``window`` [slots, taps, C] float32 is the ring of every sequence's last inputs (position p's
+    row is row p % taps) and is updated; ``meta`` gives query_start, seq_lens, state_slots (no slot twice) and max_query_len.  Nothing
+    comes before position 0; rows of a sequence without a slot become zeros, rows behind the last sequence are left as they are."""
+    _check_recurrent(meta, window, "window")
+    T, C = x.shape
+    if w.shape[0] != C or w.shape[1] < 1 or tuple(window.shape[1:]) != (w.shape[1], C) or (bias is not None and tuple(bias.shape) != (C,)):
+        raise ValueError(f"convolution of {C} channels: w {tuple(w.shape)}, window {tuple(window.shape)}"
+                         + ("" if bias is None else f", bias {tuple(bias.shape)}"))
+    if act not in ("silu", "none"):
+        raise ValueError(f"act is 'silu' or 'none', not {act!r}")
+    if x.is_cuda:
+        return _cuda_ssm().causal_conv(x, w, bias, meta, window, act, act_dtype, out)
+    y = ref.causal_conv(x, w, bias, meta, window, act, act_dtype)
+    return y if out is None else _into(out, y, meta)
+
+
+@instrument("selective_scan")
+def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype=torch.float32, out=None):
+    """Selective state-space recurrence over a step's rows, each sequence from its own state: s = softplus(dt + dt_bias);
+    h <- exp(s a) h + s u b; y = (h . c + d u) silu(z) in ``act_dtype``.  u, dt, z [T, C] and b, c [T, N] (bfloat16 or float32, possibly
+    columns of wider projections; z None: no gate); a [C, N], d [C], dt_bias [C] float32 (d, dt_bias None: zeros); ``state`` [slots, C,
+    N] float32 is updated.  ``meta`` as for ``causal_conv``.  A sequence whose rows start at position 0 starts from nothing; rows of
+    one without a slot become zeros, rows behind the last sequence are left as they are.  A sequence's result does not depend on
+    the portions that its rows come in, nor on its neighbours."""
+    _check_recurrent(meta, state, "state")
+    T, C = u.shape
+    N = a.shape[1]
+    if (tuple(dt.shape) != (T, C) or tuple(a.shape) != (C, N) or tuple(b.shape) != (T, N) or tuple(c.shape) != (T, N)
+            or tuple(state.shape[1:]) != (C, N) or (z is not None and tuple(z.shape) != (T, C))
+            or any(v is not None and tuple(v.shape) != (C,) for v in (d, dt_bias))):
+        raise ValueError(f"scan of {T} rows, {C} channels and {N} states: dt {tuple(dt.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}, "
+                         f"c {tuple(c.shape)}, state {tuple(state.shape)}")
+    if u.is_cuda:
+        return _cuda_ssm().selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype, out)
+    y = ref.selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype)
+    return y if out is None else _into(out, y, meta)
+
+
+def _check_recurrent(meta, kept, what):
+    if meta.state_slots is None:
+        raise ValueError("a layer with a recurrent state needs the sequences' state slots")
+    if kept.dtype != torch.float32 or kept.dim() != 3:
+        raise ValueError(f"{what} is float32 with three dimensions, not {kept.dtype} {tuple(kept.shape)}")
+
+
+def _into(out, y, meta):
+    n = int(meta.query_start[-1])
+    out[:n] = y[:n]
+    return out
 
 
 @instrument("gated_ffn")

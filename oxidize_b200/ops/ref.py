@@ -26,6 +26,8 @@ def dequantize_weight(w) -> torch.Tensor:
     """QTensor -> dense float32 [out, in] (host decode through the NumPy oracle)."""
     if w.qtype in ("F32", "F16", "BF16"):
         return w.data.float()
+    if w.qtype == "I8":
+        return w.data.float() * w.scales[:, None]
     if w.qtype == "FP8B":
         codes = w.data.cpu().numpy().reshape(-1)
         scales = w.scales.float().cpu().numpy().reshape(-1)
@@ -36,7 +38,29 @@ def dequantize_weight(w) -> torch.Tensor:
     return torch.from_numpy(qref.dequantize(w.qtype, raw, n).copy()).reshape(w.shape).to(w.data.device)
 
 
+def quantize_tokens(x: torch.Tensor):
+    """Rows as 8-bit integers: (codes rint(127 x / max|x|) as float64, scales max|x| / 127 as float32).  A row of zeros has the
+    scale 0, one that holds an infinity or NaN the scale NaN and codes 0."""
+    xd = x.double()
+    most = xd.abs().amax(-1, keepdim=True) if x.shape[-1] else xd.new_zeros(x.shape[0], 1)
+    fine = torch.isfinite(most)
+    codes = torch.where(fine & (most > 0), torch.round(xd * 127 / torch.where(most > 0, most, 1.0)), 0.0)
+    return codes, torch.where(fine, most.float() / 127, torch.nan).float()
+
+
+def linear_int8(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """x @ W^T on 8-bit integers (``w``: codes [out, in] with a scale per row; ``x`` gets one per token): whole-number sums, scaled
+    and rounded once."""
+    codes, scale = quantize_tokens(x)
+    y = (codes @ w.data.double().t()).float() * scale * w.scales
+    if bias is not None:
+        y = y + bias.float()
+    return y.to(x.dtype)
+
+
 def linear(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    if w.qtype == "I8":
+        return linear_int8(x, w, bias)
     dense = w.dense_cache()
     y = x.float() @ dense.t()
     if bias is not None:
@@ -484,6 +508,56 @@ def add_normed(res: torch.Tensor, y, w: torch.Tensor, groups: int, eps: float, a
         streams.n += 1
         x = depth[0] * streams.first + torch.einsum("l,lth->th", depth[1:], streams.results[: streams.n])
     return x, None if act_dtype is None else x.to(act_dtype)
+
+
+def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], meta, window: torch.Tensor, act: str,
+                act_dtype: torch.dtype) -> torch.Tensor:
+    """Short depthwise convolution over each sequence's rows, act(sum_i w[c, i] x[t - (taps - 1) + i, c] + bias[c]): x [T, C],
+    w [C, taps], ``window`` [slots, taps, C] the ring of a sequence's last inputs (position p's row is row p % taps; updated).
+    Nothing comes before position 0; a sequence without a slot gives zeros."""
+    n = w.shape[1]
+    y = torch.zeros(x.shape, dtype=torch.float32, device=x.device)
+    xf, wf = x.float(), w.float()
+    qs, lens, slots = meta.query_start.tolist(), meta.seq_lens.tolist(), meta.state_slots.tolist()
+    for b in range(len(lens)):
+        t0, t1 = qs[b], qs[b + 1]
+        m, ring = t1 - t0, window[slots[b]]
+        if slots[b] < 0 or m == 0:
+            continue
+        pos0 = lens[b] - m
+        past = torch.stack([ring[p % n] if p >= 0 else torch.zeros_like(ring[0]) for p in range(pos0 - n + 1, pos0)] or [ring[0]])
+        rows = torch.cat([past[: n - 1], xf[t0:t1]])
+        conv = sum(wf[:, j] * rows[j : j + m] for j in range(n))
+        if bias is not None:
+            conv = conv + bias.float()
+        y[t0:t1] = torch.nn.functional.silu(conv) if act == "silu" else conv
+        for p in range(max(pos0, pos0 + m - n), pos0 + m):
+            ring[p % n] = xf[t0 + p - pos0]
+    return y.to(act_dtype)
+
+
+def selective_scan(u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.Tensor, c: torch.Tensor, d: Optional[torch.Tensor],
+                   z: Optional[torch.Tensor], dt_bias: Optional[torch.Tensor], meta, state: torch.Tensor,
+                   act_dtype: torch.dtype) -> torch.Tensor:
+    """Selective state-space recurrence, token by token: s = softplus(dt + dt_bias); h <- exp(s a) h + s u b; y = (h c + d u) silu(z).
+    u, dt, z [T, C]; b, c [T, N]; a [C, N]; d, dt_bias [C]; ``state`` [slots, C, N] (updated).  A sequence whose rows start at
+    position 0 starts from nothing; one without a slot gives zeros."""
+    step = dt.float() if dt_bias is None else dt.float() + dt_bias.float()
+    step, uf, af, bf, cf = torch.nn.functional.softplus(step), u.float(), a.float(), b.float(), c.float()
+    y = torch.zeros(u.shape, dtype=torch.float32, device=u.device)
+    qs, lens, slots = meta.query_start.tolist(), meta.seq_lens.tolist(), meta.state_slots.tolist()
+    for i in range(len(lens)):
+        t0, t1 = qs[i], qs[i + 1]
+        if slots[i] < 0 or t1 == t0:
+            continue
+        h = torch.zeros_like(state[slots[i]]) if lens[i] == t1 - t0 else state[slots[i]]
+        for t in range(t0, t1):
+            h = torch.exp(af * step[t][:, None]) * h + (step[t] * uf[t])[:, None] * bf[t][None, :]
+            y[t] = h @ cf[t] + (0 if d is None else d.float() * uf[t])
+        state[slots[i]] = h
+    if z is not None:
+        y = y * torch.nn.functional.silu(z.float())
+    return y.to(act_dtype)
 
 
 def token_shift(x: torch.Tensor, mu: torch.Tensor, meta, window: torch.Tensor) -> torch.Tensor:
