@@ -20,6 +20,7 @@ import torch
 
 from ..formats.gguf import GGUFFile, GGMLTypeInfo, ggml_type
 from ..quant import ref as qref
+from ..quant import torch_quant
 from .config import ModelConfig
 
 
@@ -29,7 +30,8 @@ class QTensor:
 
     ``data`` is ``[out, in]`` for F32/F16/BF16 and ``uint8 [out, row_bytes]`` for block
     formats.  ``FP8B`` is our block-scaled fp8 (e4m3 codes + one f32 scale per ``block``
-    input channels), which has no GGUF id."""
+    input channels), ``I8`` int8 codes with one f32 scale per output channel (``scales`` [out]; rows start
+    on 16-byte boundaries), for products whose activations become 8-bit integers too; neither has a GGUF id."""
 
     qtype: str
     data: torch.Tensor
@@ -65,7 +67,10 @@ class QTensor:
         return self._dense
 
     def to(self, device) -> "QTensor":
-        return QTensor(self.qtype, self.data.to(device), self.shape,
+        data = self.data.to(device)
+        if self.qtype == "I8":
+            data = torch_quant.int8_rows(data)
+        return QTensor(self.qtype, data, self.shape,
                        None if self.scales is None else self.scales.to(device), self.block)
 
     def rows(self, start: int, stop: int) -> "QTensor":
@@ -84,6 +89,9 @@ def qtensor_from_dense(w: torch.Tensor, qtype: str = "BF16", device=None) -> QTe
         return QTensor("BF16", w.to(torch.bfloat16).to(dev).contiguous(), (out_f, in_f))
     if qtype == "F16":
         return QTensor("F16", w.to(torch.float16).to(dev).contiguous(), (out_f, in_f))
+    if qtype == "I8":
+        codes, scales = torch_quant.quantize_int8(w)
+        return QTensor("I8", torch_quant.int8_rows(codes.to(dev)), (out_f, in_f), scales.to(dev))
     x = w.detach().float().cpu().numpy()
     if qtype == "FP8B":
         codes, scales = qref.quantize_fp8_block(x.reshape(-1), 128)
@@ -117,7 +125,7 @@ class LinearWeight:
 
 
 # weight encodings the sm_100a kernels read directly (ops/cuda.py::QTYPE_CODE + the fp8-block path)
-DEVICE_PACKED_TYPES = ("F32", "F16", "BF16", "Q8_0", "Q4_0", "Q4_K", "Q5_K", "Q6_K", "NVFP4", "FP8B")
+DEVICE_PACKED_TYPES = ("F32", "F16", "BF16", "Q8_0", "Q4_0", "Q4_K", "Q5_K", "Q6_K", "NVFP4", "FP8B", "I8")
 
 
 def fuse_rows(parts: Sequence[QTensor]) -> List[QTensor]:
@@ -126,6 +134,10 @@ def fuse_rows(parts: Sequence[QTensor]) -> List[QTensor]:
     for p in parts:
         if out and out[-1].qtype == p.qtype and out[-1].in_features == p.in_features and p.qtype != "FP8B":
             a = out[-1]
+            if p.qtype == "I8":
+                out[-1] = QTensor("I8", torch_quant.int8_rows(torch.cat([a.data, p.data], 0)),
+                                  (a.out_features + p.out_features, a.in_features), torch.cat([a.scales, p.scales]))
+                continue
             out[-1] = QTensor(a.qtype, torch.cat([a.data, p.data], 0).contiguous(),
                               (a.out_features + p.out_features, a.in_features))
         else:

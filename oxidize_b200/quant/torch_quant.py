@@ -133,6 +133,24 @@ def quantize_fp8_block(w: torch.Tensor, block: int = 128):
     return codes, scale.squeeze(-1).contiguous()
 
 
+def quantize_int8(w: torch.Tensor):
+    """Rows as int8 codes with one scale each: (codes [out, in], scales [out] = max|w| / 127)."""
+    wf = w.detach().float()
+    scales = wf.abs().amax(1) / 127.0
+    codes = torch.round(wf / torch.where(scales > 0, scales, torch.ones_like(scales))[:, None]).clamp(-127, 127).to(torch.int8)
+    return codes, scales
+
+
+def int8_rows(codes: torch.Tensor) -> torch.Tensor:
+    """int8 codes [out, in] with rows on 16-byte boundaries (a copy where they are not)."""
+    n, k = codes.shape
+    if codes.stride(1) == 1 and codes.stride(0) % 16 == 0 and codes.stride(0) >= k and codes.data_ptr() % 16 == 0:
+        return codes
+    rows = torch.zeros(n, -(-k // 16) * 16, dtype=torch.int8, device=codes.device)[:, :k]
+    rows.copy_(codes)
+    return rows
+
+
 def random_quantized(out_f: int, in_f: int, qtype: str, device, gen: torch.Generator, std: float):
     """N(0, std) weight encoded as ``qtype``, generated and encoded in row chunks on ``device``."""
     from ..models.weights import QTensor
@@ -146,6 +164,13 @@ def random_quantized(out_f: int, in_f: int, qtype: str, device, gen: torch.Gener
             w = torch.empty(min(step, out_f - r), in_f, device=device).normal_(0.0, std, generator=gen)
             codes[r : r + step], scales[r : r + step] = quantize_fp8_block(w)
         return QTensor("FP8B", codes, (out_f, in_f), scales, 128)
+    if qtype == "I8":
+        codes = torch.zeros(out_f, -(-in_f // 16) * 16, dtype=torch.int8, device=device)[:, :in_f]
+        scales = torch.empty(out_f, dtype=torch.float32, device=device)
+        for r in range(0, out_f, step):
+            w = torch.empty(min(step, out_f - r), in_f, device=device).normal_(0.0, std, generator=gen)
+            codes[r : r + step], scales[r : r + step] = quantize_int8(w)
+        return QTensor("I8", codes, (out_f, in_f), scales)
     t = ggml_type(qtype)
     data = torch.empty(out_f, in_f // t.block_size * t.type_size, dtype=torch.uint8, device=device)
     for r in range(0, out_f, step):
