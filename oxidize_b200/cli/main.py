@@ -55,7 +55,7 @@ def rewrite_args(argv: List[str]) -> List[str]:
 _BOOL_FLAGS = {"--chat", "--cpu-optimized", "--ram-offload", "--mmap-prefetch", "--mmap-hugepages", "--layer-wise",
                "--turboquant-kv", "--no-turboquant-kv", "--mesh", "--auto", "--no-auto", "--no-api", "--serve-api",
                "--api-only", "--vision", "--force-dflash", "--no-mtp", "--quantspec", "--pipe-head", "--pipe-tail",
-               "--turboquant", "--no-turboquant", "--json", "--bench-no-eos", "--cuda-graphs", "--no-cuda-graphs"}
+               "--turboquant", "--no-turboquant", "--int8", "--json", "--bench-no-eos", "--cuda-graphs", "--no-cuda-graphs"}
 
 
 def build_parser() -> argparse.ArgumentParser:
@@ -87,6 +87,7 @@ def build_parser() -> argparse.ArgumentParser:
     a("--turboquant", action="store_true", help="re-encode float weight matrices as block-wise int8 (Q8_0) while loading")
     a("--turboquant-bits", type=int, default=8, choices=[4, 8])
     a("--no-turboquant", action="store_true")
+    a("--int8", action="store_true", help="run float projections as products on 8-bit integers (a scale per output channel and per token)")
     a("--threads", type=int, default=0)
     a("--n-gpu-layers", type=int, default=0)
     a("--gpus", type=int, default=0)
@@ -275,6 +276,8 @@ def make_engine(args, passed: set, device_index: Optional[int] = None):
     if kvd == "auto":
         # (latent cache rows of a layer-list model are kept in the compute type: the engine's own choice)
         kvd = plan.kv_cache_dtype if (use_plan and backend == plan.backend and not isinstance(g, LayeredCheckpoint)) else "auto"
+    if args.int8 and args.turboquant and not args.no_turboquant:
+        raise SystemExit("error: --int8 and --turboquant are two encodings of the same weights")
     tp = args.tp or (args.gpus if args.parallelism == "tensor" and args.gpus > 1 else 0) or 1
     ec = EngineConfig(kv_cache_dtype=kvd, kv_page_size=args.kv_page_size,
                       max_model_len=args.ctx_size or plan.ctx_size, max_num_seqs=args.max_running or plan.max_num_seqs,
@@ -282,7 +285,7 @@ def make_engine(args, passed: set, device_index: Optional[int] = None):
                       compute_dtype=args.compute_dtype, cuda_graphs=not args.no_cuda_graphs, tp_size=tp, ep_size=args.ep or tp, pp_size=max(1, args.pp),
                       fused_comm=args.fused_comm == "on",
                       resident_layers=max(1, args.layer_cache) if args.layer_wise else 0,
-                      weight_transcode=("Q4_0" if args.turboquant_bits == 4 else "Q8_0")
+                      weight_transcode="I8" if args.int8 else ("Q4_0" if args.turboquant_bits == 4 else "Q8_0")
                       if (args.turboquant and not args.no_turboquant) else "")
     if args.ram_offload and not args.layer_wise:
         # keep as many layers loaded as fit beside the cache, stream the rest from the file mapping

@@ -65,7 +65,9 @@ class EngineConfig:
     # reaches them (for checkpoints larger than the memory left beside the KV cache)
     resident_layers: int = 0
     # "Q8_0" / "Q4_0": float weight matrices are re-encoded in that block format while loading (the reference's
-    # --turboquant: block-wise int8 / int4 weights with per-block scales); "" = keep the checkpoint's encodings
+    # --turboquant: block-wise int8 / int4 weights with per-block scales); "I8": float projections become int8 rows with a scale
+    # per output channel and run as products on 8-bit integers (activations get a scale per token); "" = keep the
+    # checkpoint's encodings
     weight_transcode: str = ""
 
 

@@ -416,12 +416,20 @@ def _np_to_torch(a: np.ndarray, device, dtype=None) -> torch.Tensor:
     return t.to(device)
 
 
+# Projections that run as products on 8-bit integers when asked for ("I8"): those that are most of a layer's bytes.  Embeddings, the
+# head, routers, routed experts and the narrow projections that steer a recurrence or make latent rows stay as they are stored.
+INT8_PROJECTIONS = frozenset(f"{n}.weight" for n in (
+    "attn_q", "attn_k", "attn_v", "attn_qkv", "attn_gate", "attn_output", "ffn_gate", "ffn_up", "ffn_down", "ffn_gate_shexp", "ffn_up_shexp",
+    "ffn_down_shexp", "ssm_in", "ssm_out", "shortconv.in_proj", "shortconv.out_proj"))
+
+
 class GGUFWeightSource:
     """Reads (slices of) tensors from a GGUF mapping into device QTensors."""
 
     def __init__(self, g: GGUFFile, device, act_dtype: torch.dtype, transcode: str = ""):
         self.g = g
-        # "Q8_0" / "Q4_0": weight matrices stored as floats are re-encoded in that block format on the way in
+        # "Q8_0" / "Q4_0": weight matrices stored as floats are re-encoded in that block format on the way in; "I8": the
+        # projections among them (INT8_PROJECTIONS) as int8 rows
         self.transcode = transcode.upper()
         self.device = torch.device(device)
         self.act_dtype = act_dtype
@@ -454,7 +462,13 @@ class GGUFWeightSource:
                 raise ValueError(f"{name}: column shard [{c0},{c1}) not on {t.name} block boundary {t.block_size}")
             raw = raw[:, c0 // t.block_size * t.type_size : c1 // t.block_size * t.type_size]
         new_shape = (r1 - r0, c1 - c0)
-        if (self.transcode and t.name in ("F32", "F16", "BF16") and new_shape[1] % 32 == 0 and new_shape[0] > 1
+        if self.transcode == "I8":
+            if t.name in ("F32", "F16", "BF16") and len(shape) == 2 and name.split(".", 2)[-1] in INT8_PROJECTIONS:
+                x = qref.dequantize(t.name, np.ascontiguousarray(raw).reshape(-1), new_shape[0] * new_shape[1])
+                w = _np_to_torch(np.asarray(x, dtype=np.float32).reshape(new_shape), self.device)
+                codes, scales = torch_quant.quantize_int8(w)
+                return QTensor("I8", torch_quant.int8_rows(codes), new_shape, scales)
+        elif (self.transcode and t.name in ("F32", "F16", "BF16") and new_shape[1] % 32 == 0 and new_shape[0] > 1
                 and "token_embd" not in name and "ffn_gate_inp" not in name):
             x = qref.dequantize(t.name, np.ascontiguousarray(raw).reshape(-1), new_shape[0] * new_shape[1])
             tt = ggml_type(self.transcode)
@@ -644,8 +658,8 @@ def load_weights(g: GGUFFile, cfg: ModelConfig, device="cpu", act_dtype: torch.d
     ``layer_range`` selects a pipeline stage (only its own tensors are read, unlike the
     reference's two-node pipeline where both nodes map the whole file, pipeline.rs:23).
     ``resident_layers`` > 0 keeps only that many decoder layers loaded at a time (:class:`StreamedLayers`)."""
-    if transcode and transcode.upper() not in ("Q8_0", "Q4_0"):
-        raise ValueError("weights can be re-encoded at load time as Q8_0 or Q4_0")
+    if transcode and transcode.upper() not in ("Q8_0", "Q4_0", "I8"):
+        raise ValueError("weights can be re-encoded at load time as Q8_0, Q4_0 or I8")
     src = GGUFWeightSource(g, device, act_dtype, transcode)
     l0, l1 = layer_range if layer_range is not None else (0, cfg.n_layers)
     if resident_layers > 0 and resident_layers < l1 - l0:
