@@ -20,8 +20,8 @@ def lib():
     L = opcuda.lib()
     if not _declared:
         vp, i32, i64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
-        L.oxb_causal_conv.argtypes = [vp, i32, i32] + [vp] * 6 + [i64, i32, vp] + [i32] * 7 + [vp]
-        L.oxb_selective_scan.argtypes = [vp, i32, i32] * 5 + [vp] * 7 + [i64, i32, vp] + [i32] * 6 + [vp]
+        L.oxb_causal_conv.argtypes = [vp, i32, i32] + [vp] * 6 + [i64, i32, vp] + [i32] * 8 + [vp]
+        L.oxb_selective_scan.argtypes = [vp, i32, i32] * 5 + [vp] * 7 + [i64, i32, vp] + [i32] * 7 + [vp]
         _declared = True
     return L
 
@@ -65,7 +65,7 @@ def causal_conv(x, w, bias, meta, window, act, act_dtype, out=None):
     _check(lib().oxb_causal_conv(x.data_ptr(), x.stride(0), DT[x.dtype], w.data_ptr(), _p(bias), meta.query_start.data_ptr(),
                                  meta.seq_lens.data_ptr(), meta.state_slots.data_ptr(), window.data_ptr(), window.stride(0), window.shape[0],
                                  y.data_ptr(), y.stride(0), DT[act_dtype], meta.seq_lens.shape[0], T, C, w.shape[1], int(act == "silu"),
-                                 _stream()), "oxb_causal_conv")
+                                 meta.max_query_len, _stream()), "oxb_causal_conv")
     return y
 
 
@@ -81,6 +81,6 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype, out=No
     at = lambda m: (m.data_ptr(), m.stride(0), DT[m.dtype])  # noqa: E731
     _check(lib().oxb_selective_scan(*at(u), *at(dt), *((None, 0, 0) if z is None else at(z)), *at(b), *at(c), a.data_ptr(), _p(d),
                                     _p(dt_bias), meta.query_start.data_ptr(), meta.seq_lens.data_ptr(), meta.state_slots.data_ptr(),
-                                    state.data_ptr(), state.stride(0), state.shape[0], *at(y), meta.seq_lens.shape[0], T, C, N, _stream()),
+                                    state.data_ptr(), state.stride(0), state.shape[0], *at(y), meta.seq_lens.shape[0], T, C, N, meta.max_query_len, _stream()),
            "oxb_selective_scan")
     return y

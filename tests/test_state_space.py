@@ -444,3 +444,24 @@ def test_long_sequences_and_many():
         y1[take] = ops.causal_conv(x[take], w, None, one, win1)
         s1[take] = ops.selective_scan(**{k: m[take] if k in ("u", "dt", "b", "c", "z") else m for k, m in v.items()}, meta=one, state=state1)
     assert torch.equal(y, y1) and torch.equal(win, win1) and torch.equal(s, s1) and torch.equal(state, state1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lens", [[1, 1, 1], [4, 1, 2]])
+def test_slots_outside_the_store_are_reported(lens):
+    """Such a sequence's rows become zeros, nothing is written for it, the status word names its slot."""
+    from oxidize_b200.ops import cuda as C
+
+    gen = torch.Generator().manual_seed(23)
+    meta = step(lens, "cuda", slots=(1, 77, 0))
+    T = sum(lens)
+    v = scan_inputs(gen, T, 40, 16, "f32", "f32", "f32", "f32", True, True, True, 0, "cuda")
+    w, window, state = torch.randn(40, 4, generator=gen).cuda(), torch.randn(3, 4, 40, generator=gen).cuda(), torch.randn(3, 40, 16, generator=gen).cuda()
+    kept = window[2].clone(), state[2].clone()
+    C.status()
+    y = ops.causal_conv(v["u"], w, None, meta, window)
+    assert C.status()[:2] == (6 + 1, 77)
+    s = ops.selective_scan(**v, meta=meta, state=state)
+    assert C.status()[:2] == (6 + 1, 77)
+    mine = slice(lens[0], lens[0] + lens[1])
+    assert (y[mine] == 0).all() and (s[mine] == 0).all() and torch.equal(window[2], kept[0]) and torch.equal(state[2], kept[1])
