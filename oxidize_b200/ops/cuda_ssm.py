@@ -75,6 +75,8 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype, out=No
     if not 1 <= N <= MAX_STATES:
         raise ValueError(f"the scan takes 1 to {MAX_STATES} states, not {N}")
     u, dt, b, c = _rows(u, "u"), _rows(dt, "dt"), _rows(b, "b"), _rows(c, "c")
+    if u.dtype != dt.dtype:  # (the kernels read them as one type)
+        u, dt = u.float(), dt.float()
     z = None if z is None else _rows(z, "z")
     a, d, dt_bias, state = _floats(a, "a"), _floats(d, "d"), _floats(dt_bias, "dt_bias"), _kept(state, "state")
     y = _out(out, T, C, act_dtype, u.device)
