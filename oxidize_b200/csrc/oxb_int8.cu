@@ -3,52 +3,106 @@
 #include "gemm_int8.cuh"
 using namespace oxb;
 
-// Rows of x [T, K] bf16 as int8 codes q (rows ld_q >= K bytes apart) with a scale per row
-OXB_API int oxb_quantize_tokens(const void* x, int T, int K, void* q, int ld_q, float* scales, cudaStream_t stream) {
-  if (T <= 0) return 0;
-  if (K <= 0 || ld_q < K) return (int)cudaErrorInvalidValue;
-  oxb_launch(quantize_tokens_kernel, dim3(T), dim3(256), 0, stream, reinterpret_cast<const __nv_bfloat16*>(x), K, reinterpret_cast<int8_t*>(q),
-             ld_q, scales);
-  OXB_CHECK_LAUNCH();
-  return 0;
-}
-
-template <int TN>
-static int int8_go(const CUtensorMap& tw, const CUtensorMap& tx, const I8Args& a, cudaStream_t stream) {
-  static bool configured[64] = {false};
+// Attributes of a kernel, set once per device; 0 or an error
+template <typename F>
+static int int8_configure(F* kernel, int smem, bool (&done)[64]) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64) return (int)cudaErrorInvalidDevice;
-  if (!configured[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(gemm_int8_kernel<TN>, cudaFuncAttributeMaxDynamicSharedMemorySize, I8Tile<TN>::SMEM);
+  if (!done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return (int)e;
-    configured[dev] = true;
+    done[dev] = true;
   }
-  const dim3 grid((a.N + I8_BM - 1) / I8_BM, 1, (a.T + TN - 1) / TN);
-  if (grid.z > 65535) return (int)cudaErrorInvalidValue;
-  const cudaError_t e = oxb_launch(gemm_int8_kernel<TN>, grid, dim3(I8_THREADS), (size_t)I8Tile<TN>::SMEM, stream, tw, tx, a);
-  if (e != cudaSuccess) return (int)e;
-  OXB_CHECK_LAUNCH();
   return 0;
 }
 
-// Y [T, N] bf16 (rows ld_y apart) from int8 codes xq [T, K] and w [N, K] (rows on 16-byte boundaries, ld bytes apart) with scales per
-// row; bias [N] or null.  The sums are 32-bit: K <= 131072.
-OXB_API int oxb_gemm_int8(const void* xq, int ld_x, const float* sx, const void* w, int ld_w, const float* sw, const float* bias, void* y,
-                          int ld_y, int T, int N, int K, cudaStream_t stream) {
-  if (T <= 0 || N <= 0) return 0;
-  if (K <= 0 || K > 131072 || ld_y < N) return (int)cudaErrorInvalidValue;
-  const int tn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
-  CUtensorMap tw, tx;
-  int e = oxb_make_tmap_2d(&tw, w, N, K, ld_w, I8_BM, I8_BK, 1);
-  if (!e) e = oxb_make_tmap_2d(&tx, xq, T, K, ld_x, tn, I8_BK, 1);
+static int quantize_launch(const __nv_bfloat16* x, int T, int K, int8_t* q, int ld_q, float* scales, cudaStream_t stream) {
+  const int wide = K % 8 == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+  const cudaError_t e = K <= 4096   ? oxb_launch(quantize_tokens_kernel<2>, dim3(T), dim3(256), 0, stream, x, K, wide, q, ld_q, scales)
+                        : K <= 8192 ? oxb_launch(quantize_tokens_kernel<4>, dim3(T), dim3(256), 0, stream, x, K, wide, q, ld_q, scales)
+                                    : oxb_launch(quantize_tokens_kernel<8>, dim3(T), dim3(256), 0, stream, x, K, wide, q, ld_q, scales);
+  return (int)e;
+}
+
+template <int TN, int RB = 1>
+static int int8_go(const CUtensorMap& tw, const CUtensorMap& tx, const I8Args& a, int splits, cudaStream_t stream) {
+  static bool done[64] = {false};
+  const int e = int8_configure(gemm_int8_kernel<TN, RB>, I8Tile<TN, RB>::SMEM, done);
   if (e) return e;
-  const I8Args a{reinterpret_cast<__nv_bfloat16*>(y), sx, sw, bias, N, T, K, ld_y, N % 8 == 0 && ld_y % 8 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0};
-  switch (tn) {
-    case 16: return int8_go<16>(tw, tx, a, stream);
-    case 32: return int8_go<32>(tw, tx, a, stream);
-    case 64: return int8_go<64>(tw, tx, a, stream);
-    case 128: return int8_go<128>(tw, tx, a, stream);
-    default: return int8_go<256>(tw, tx, a, stream);
+  const dim3 grid((a.N + RB * I8_BM - 1) / (RB * I8_BM), splits, (a.T + TN - 1) / TN);
+  if (grid.z > 65535) return (int)cudaErrorInvalidValue;
+  return (int)(splits > 1 ? oxb_launch_cluster(gemm_int8_kernel<TN, RB>, grid, dim3(I8_THREADS), dim3(1, splits, 1), (size_t)I8Tile<TN, RB>::SMEM, stream, tw, tx, a)
+                          : oxb_launch(gemm_int8_kernel<TN, RB>, grid, dim3(I8_THREADS), (size_t)I8Tile<TN, RB>::SMEM, stream, tw, tx, a));
+}
+
+// Tokens and blocks of 128 weight rows of a tile, CTAs that share its K
+struct I8Plan {
+  int tn, rb, splits;
+};
+static I8Plan int8_plan(int T, int N, int K) {
+  const int sms = oxb_sm_count(), n_tiles = (N + 127) / 128, kbs = (K + I8_BK - 1) / I8_BK;
+  if (T > 128) {
+    // One CTA to an SM, in waves.  A tile's time in those of 128 x 256: 128 x 128 0.62, 256 x 256 1.75 (us with the three, 128 x 128
+    // first: 512 tokens of 4096 x 4096 17.5, 22.4, 38; 1024 of 4096 x 4096 32, 26, 40; 1024 of 14336 x 4096 96, 84, 76; 8192 of
+    // 8192 x 8192 623, 575, 474).
+    auto waves = [&](int rows, int tokens) { return (int)(((long long)((N + rows - 1) / rows) * ((T + tokens - 1) / tokens) + sms - 1) / sms); };
+    const double w1 = 0.62 * waves(128, 128), w2 = waves(128, 256), w4 = 1.75 * waves(256, 256);
+    return w4 <= w2 && w4 <= w1 ? I8Plan{256, 2, 1} : w2 <= w1 ? I8Plan{256, 1, 1} : I8Plan{128, 1, 1};
   }
+  const int tn = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : 128;
+  // Splits: as many as the SMs hold at a time (two CTAs of up to 64 tokens each), of 8 k-blocks and more; none where the weight tiles
+  // alone nearly fill the SMs.  us with 1, 2, 4, 8: 16 tokens of 4096 x 14336 35, 22, 17, 16; 64 of 4096 x 4096 11.8, 12.0, 10.4,
+  // 11.8; of 8192 x 8192 25, 21, 19, 29; of 14336 x 4096 16.4, 18.0, 25, 39.  128 tokens: large sums, so only for few tiles (4096 x 4096
+  // 13.9, 16.9, 15.2, 36).
+  int splits = 1;
+  if (4 * n_tiles <= 3 * sms) splits = tn <= 64 ? 2 * sms / n_tiles : sms / (4 * n_tiles);
+  splits = splits < kbs / 8 ? splits : kbs / 8;
+  return {tn, 1, splits < 1 ? 1 : splits > 8 ? 8 : splits};
+}
+
+// Y [T, N] bf16 (rows ld_y apart) from x [T, K] bf16 (contiguous) and int8 codes w [N, K] (rows on 16-byte boundaries, ld_w bytes apart)
+// with scales per row; bias [N] or null.  The sums are 32-bit: K <= 131072.  rows: scratch of T rows of K codes, each padded to 16 bytes, and
+// T float scales behind them (may be null where oxb_int8_needs_rows is 0: one token of up to 40960 values); quantized: they are there from an
+// earlier call on the same x.
+OXB_API int oxb_int8_needs_rows(int T, int K) { return T > 1 || K > 40960; }
+OXB_API int oxb_linear_int8(const void* x, int T, int K, void* rows, int quantized, const void* w, int ld_w, const float* sw, const float* bias,
+                            void* y, int ld_y, int N, cudaStream_t stream) {
+  if (T <= 0 || N <= 0) return 0;
+  if (K <= 0 || K > 131072 || ld_y < N || ld_w % 16 != 0 || (reinterpret_cast<uintptr_t>(w) & 15) != 0) return (int)cudaErrorInvalidValue;
+  const __nv_bfloat16* xb = reinterpret_cast<const __nv_bfloat16*>(x);
+  __nv_bfloat16* yb = reinterpret_cast<__nv_bfloat16*>(y);
+  int e = 0;
+  if (!oxb_int8_needs_rows(T, K)) {
+    const int wide = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    e = (int)oxb_launch(gemv_int8_kernel<4>, dim3((N + 31) / 32), dim3(256), (size_t)((K + 511) / 512 * 512), stream, xb, wide,
+                        reinterpret_cast<const int8_t*>(w), ld_w, sw, bias, yb, N, K);
+    if (e) return e;
+    OXB_CHECK_LAUNCH();
+    return 0;
+  }
+  if (rows == nullptr) return (int)cudaErrorInvalidValue;
+  const int ld_q = (K + 15) / 16 * 16;
+  int8_t* q = reinterpret_cast<int8_t*>(rows);
+  float* scales = reinterpret_cast<float*>(q + (size_t)T * ld_q);
+  if (!quantized) {
+    e = quantize_launch(xb, T, K, q, ld_q, scales, stream);
+    if (e) return e;
+  }
+  const I8Plan p = int8_plan(T, N, K);
+  CUtensorMap tw, tx;
+  e = oxb_make_tmap_2d(&tw, w, N, K, ld_w, I8_BM, I8_BK, 1);
+  if (!e) e = oxb_make_tmap_2d(&tx, q, T, K, ld_q, p.tn, I8_BK, 1);
+  if (e) return e;
+  const I8Args a{yb, scales, sw, bias, N, T, K, ld_y, N % 8 == 0 && ld_y % 8 == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0};
+  switch (p.tn) {
+    case 16: e = int8_go<16>(tw, tx, a, p.splits, stream); break;
+    case 32: e = int8_go<32>(tw, tx, a, p.splits, stream); break;
+    case 64: e = int8_go<64>(tw, tx, a, p.splits, stream); break;
+    case 128: e = int8_go<128>(tw, tx, a, p.splits, stream); break;
+    default: e = p.rb == 2 ? int8_go<256, 2>(tw, tx, a, 1, stream) : int8_go<256>(tw, tx, a, 1, stream); break;
+  }
+  if (e) return e;
+  OXB_CHECK_LAUNCH();
+  return 0;
 }

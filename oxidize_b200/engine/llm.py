@@ -127,7 +127,7 @@ class LLM:
                                   and isinstance(weights.layers, list)  # a captured graph would pin evicted layers' addresses
                                   and not self.cfg.is_mla  # latent attention's device step sizes its gather on the host
                                   and not self.model.n_conv_layers  # so does the convolution layers' row gather
-                                  and not self.cfg.is_ssm)  # the recurrence runs from the host, token by token
+                                  and not self.cfg.is_ssm)  # the host looks up the sequences' state slots
         self.eos_token_id = c.eos_token_id
         if self.eos_token_id is None and tokenizer is not None:
             self.eos_token_id = tokenizer.special_tokens.eos

@@ -362,7 +362,7 @@ def linear(x: torch.Tensor, parts: Sequence, bias: Optional[torch.Tensor] = None
     N = sum(p.shape[0] for p in parts)
     if out is None:
         out = torch.empty(T, N, dtype=torch.bfloat16, device=x.device)
-    off, rows = 0, None  # rows: the tokens as 8-bit integers, once for all parts
+    off, rows = 0, None  # rows: the tokens as 8-bit integers, for all parts that want them
     for p in parts:
         n = p.shape[0]
         b = None if bias is None else bias[off : off + n]
@@ -381,8 +381,7 @@ def linear(x: torch.Tensor, parts: Sequence, bias: Optional[torch.Tensor] = None
         elif p.qtype == "I8":
             from . import cuda_int8
 
-            rows = cuda_int8.quantize_tokens(x) if rows is None else rows
-            cuda_int8.linear(rows, p, view, b, out.stride(0))
+            rows = cuda_int8.linear(x, p, view, b, out.stride(0), rows)
         else:
             from . import cuda_quant
 

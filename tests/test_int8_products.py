@@ -300,3 +300,29 @@ def test_other_encodings_are_refused(tmp_path):
         _llm(path, "cpu", "I4")
     with pytest.raises(SystemExit):
         cli.main(["run", path, "hi", "--int8", "--turboquant"])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,n,k", [(1000, 5000, 300), (2049, 2300, 1000), (4096, 4096, 128), (777, 9000, 2050), (1500, 6001, 17), (257, 40000, 520)])
+def test_many_tokens(T, n, k):
+    """Many tiles, odd edges on all sides, twice in a row."""
+    from oxidize_b200.ops import cuda as C
+
+    gen = torch.Generator().manual_seed(T)
+    q = weight(gen, n, k, "cuda")
+    bias = torch.randn(n, generator=gen).cuda()
+    for _ in range(2):
+        x = torch.randn(T, k, generator=gen).bfloat16().cuda()
+        check(x, q, bias, ops.linear(x, LinearWeight([q], bias)))
+    assert C.status()[0] == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 2, 3, 5])
+@pytest.mark.parametrize("k", [16, 40959, 40976, 512, 1023])
+def test_few_tokens(T, k):
+    """Both sides of where single tokens have a kernel of their own; a matrix that ends with its last value."""
+    gen = torch.Generator().manual_seed(k)
+    q = weight(gen, 70, k, "cuda")
+    x = torch.randn(T, k, generator=gen).bfloat16().cuda()
+    check(x, q, None, ops.linear(x, LinearWeight([q])))
