@@ -239,7 +239,8 @@ def causal_conv(x, w, bias, meta, window, act="silu", act_dtype=torch.float32, o
     comes before position 0; rows of a sequence without a slot become zeros, rows behind the last sequence are left as they are."""
     _check_recurrent(meta, window, "window")
     T, C = x.shape
-    if w.shape[0] != C or w.shape[1] < 1 or tuple(window.shape[1:]) != (w.shape[1], C) or (bias is not None and tuple(bias.shape) != (C,)):
+    taps = w.shape[1]
+    if w.shape[0] != C or taps < 1 or window.shape[1:] != (taps, C) or (bias is not None and bias.shape != (C,)):
         raise ValueError(f"convolution of {C} channels: w {tuple(w.shape)}, window {tuple(window.shape)}"
                          + ("" if bias is None else f", bias {tuple(bias.shape)}"))
     if act not in ("silu", "none"):
@@ -261,9 +262,8 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype=torch.f
     _check_recurrent(meta, state, "state")
     T, C = u.shape
     N = a.shape[1]
-    if (tuple(dt.shape) != (T, C) or tuple(a.shape) != (C, N) or tuple(b.shape) != (T, N) or tuple(c.shape) != (T, N)
-            or tuple(state.shape[1:]) != (C, N) or (z is not None and tuple(z.shape) != (T, C))
-            or any(v is not None and tuple(v.shape) != (C,) for v in (d, dt_bias))):
+    if (dt.shape != (T, C) or a.shape != (C, N) or b.shape != (T, N) or c.shape != (T, N) or state.shape[1:] != (C, N)
+            or (z is not None and z.shape != (T, C)) or (d is not None and d.shape != (C,)) or (dt_bias is not None and dt_bias.shape != (C,))):
         raise ValueError(f"scan of {T} rows, {C} channels and {N} states: dt {tuple(dt.shape)}, a {tuple(a.shape)}, b {tuple(b.shape)}, "
                          f"c {tuple(c.shape)}, state {tuple(state.shape)}")
     if u.is_cuda:

@@ -154,7 +154,7 @@ def _check(code: int, what: str) -> None:
 
 def _stream() -> int:
     # (the handle alone: torch.cuda.current_stream() makes an object around it, 3 us)
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def _p(t: Optional[torch.Tensor]) -> Optional[int]:
@@ -365,8 +365,11 @@ def linear(x: torch.Tensor, parts: Sequence, bias: Optional[torch.Tensor] = None
     off, rows = 0, None  # rows: the tokens as 8-bit integers, for all parts that want them
     for p in parts:
         n = p.shape[0]
-        b = None if bias is None else bias[off : off + n]
-        view = out[:, off : off + n]
+        if n == N:  # (a view costs 2 us)
+            b, view = bias, out
+        else:
+            b = None if bias is None else bias[off : off + n]
+            view = out[:, off : off + n]
         if p.qtype == "BF16":
             xp, data = pad_k(x, p)
             gemm_bf16(xp, data, view, b, ld_out=out.stride(0))

@@ -1,4 +1,4 @@
-"""Bindings of the kernels of state-space layers (``csrc/oxb_ssm.cu``).  CUDA tensors only; see
+"""Bindings of the kernels of state-space layers (``csrc/oxb_conv.cu``, ``csrc/oxb_ssm.cu``).  CUDA tensors only; see
 :func:`oxidize_b200.ops.causal_conv` and :func:`oxidize_b200.ops.selective_scan` for the operators' meaning."""
 from __future__ import annotations
 
@@ -26,11 +26,16 @@ def lib():
     return L
 
 
-def _rows(x: torch.Tensor, what: str) -> torch.Tensor:
-    """x with neighbouring columns, in a type that the kernels read."""
-    if x.dtype not in DT:
+def _rows(x: torch.Tensor, what: str):
+    """(x with neighbouring columns, the three arguments that stand for it) in a type that the kernels read."""
+    code = DT.get(x.dtype)
+    if code is None:
         raise ValueError(f"{what} is float32 or bfloat16, not {x.dtype}")
-    return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
+    ld, one = x.stride()
+    if one != 1 and x.shape[1] != 1:
+        x = x.contiguous()
+        ld = x.stride(0)
+    return x, (x.data_ptr(), ld, code)
 
 
 def _floats(v: Optional[torch.Tensor], what: str) -> Optional[torch.Tensor]:
@@ -38,34 +43,46 @@ def _floats(v: Optional[torch.Tensor], what: str) -> Optional[torch.Tensor]:
         return None
     if v.dtype != torch.float32:
         raise ValueError(f"{what} is float32, not {v.dtype}")
-    return v.contiguous()
+    return v if v.is_contiguous() else v.contiguous()
 
 
-def _kept(v: torch.Tensor, what: str) -> torch.Tensor:
-    """Slots that the kernels update in place: each one contiguous, any distance apart."""
-    if v.stride(2) != 1 or v.stride(1) != v.shape[2]:
+def _kept(v: torch.Tensor, what: str):
+    """Slots that the kernels update in place, each one contiguous, any distance apart: address, distance, count."""
+    n, _, width = v.shape
+    step, row, one = v.stride()
+    if one != 1 or row != width:
         raise ValueError(f"a slot of {what} is contiguous; strides are {v.stride()}")
-    return v
+    return v.data_ptr(), step, n
 
 
-def _out(out: Optional[torch.Tensor], T: int, C: int, dtype: torch.dtype, device) -> torch.Tensor:
+def _sequences(meta):
+    """Query starts, lengths with this step's rows, slots, and how many sequences there are."""
+    starts, lens, slots = meta.query_start, meta.seq_lens, meta.state_slots
+    n = lens.shape[0]
+    if starts.shape[0] <= n or slots.shape[0] < n or not starts.dtype == lens.dtype == slots.dtype == torch.int32:
+        raise ValueError(f"a step of {n} sequences has that many lengths and slots and a query start more, in int32, not {starts.dtype} "
+                         f"{tuple(starts.shape)}, {lens.dtype} and {slots.dtype} {tuple(slots.shape)}")
+    return (starts.data_ptr(), lens.data_ptr(), slots.data_ptr()), n
+
+
+def _out(out: Optional[torch.Tensor], T: int, C: int, dtype: torch.dtype, like: torch.Tensor) -> torch.Tensor:
     if dtype not in DT:
         raise ValueError(f"act_dtype is float32 or bfloat16, not {dtype}")
     if out is None:
-        return torch.empty(T, C, dtype=dtype, device=device)
-    if tuple(out.shape) != (T, C) or out.dtype != dtype or (out.stride(1) != 1 and C > 1):
+        return like.new_empty((T, C), dtype=dtype)
+    if out.shape != (T, C) or out.dtype != dtype or (out.stride(1) != 1 and C > 1):
         raise ValueError(f"out is [{T}, {C}] in {dtype} with neighbouring columns, not {tuple(out.shape)} in {out.dtype}")
     return out
 
 
 def causal_conv(x, w, bias, meta, window, act, act_dtype, out=None):
-    x, w, bias, window = _rows(x, "x"), _floats(w, "w"), _floats(bias, "bias"), _kept(window, "window")
     T, C = x.shape
-    y = _out(out, T, C, act_dtype, x.device)
-    _check(lib().oxb_causal_conv(x.data_ptr(), x.stride(0), DT[x.dtype], w.data_ptr(), _p(bias), meta.query_start.data_ptr(),
-                                 meta.seq_lens.data_ptr(), meta.state_slots.data_ptr(), window.data_ptr(), window.stride(0), window.shape[0],
-                                 y.data_ptr(), y.stride(0), DT[act_dtype], meta.seq_lens.shape[0], T, C, w.shape[1], int(act == "silu"),
-                                 meta.max_query_len, _stream()), "oxb_causal_conv")
+    x, at_x = _rows(x, "x")
+    w, bias = _floats(w, "w"), _floats(bias, "bias")
+    seqs, B = _sequences(meta)
+    y = _out(out, T, C, act_dtype, x)
+    _check(lib().oxb_causal_conv(*at_x, w.data_ptr(), _p(bias), *seqs, *_kept(window, "window"), y.data_ptr(), y.stride(0), DT[act_dtype], B, T, C,
+                                 w.shape[1], act == "silu", meta.max_query_len, _stream()), "oxb_causal_conv")
     return y
 
 
@@ -74,15 +91,13 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype, out=No
     N = a.shape[1]
     if not 1 <= N <= MAX_STATES:
         raise ValueError(f"the scan takes 1 to {MAX_STATES} states, not {N}")
-    u, dt, b, c = _rows(u, "u"), _rows(dt, "dt"), _rows(b, "b"), _rows(c, "c")
-    if u.dtype != dt.dtype:  # (the kernels read them as one type)
+    if u.dtype != dt.dtype and u.dtype in DT and dt.dtype in DT:  # (the kernels read them as one type)
         u, dt = u.float(), dt.float()
-    z = None if z is None else _rows(z, "z")
-    a, d, dt_bias, state = _floats(a, "a"), _floats(d, "d"), _floats(dt_bias, "dt_bias"), _kept(state, "state")
-    y = _out(out, T, C, act_dtype, u.device)
-    at = lambda m: (m.data_ptr(), m.stride(0), DT[m.dtype])  # noqa: E731
-    _check(lib().oxb_selective_scan(*at(u), *at(dt), *((None, 0, 0) if z is None else at(z)), *at(b), *at(c), a.data_ptr(), _p(d),
-                                    _p(dt_bias), meta.query_start.data_ptr(), meta.seq_lens.data_ptr(), meta.state_slots.data_ptr(),
-                                    state.data_ptr(), state.stride(0), state.shape[0], *at(y), meta.seq_lens.shape[0], T, C, N, meta.max_query_len, _stream()),
-           "oxb_selective_scan")
+    (u, at_u), (dt, at_dt), (b, at_b), (c, at_c) = _rows(u, "u"), _rows(dt, "dt"), _rows(b, "b"), _rows(c, "c")
+    z, at_z = (None, (None, 0, 0)) if z is None else _rows(z, "z")
+    a, d, dt_bias = _floats(a, "a"), _floats(d, "d"), _floats(dt_bias, "dt_bias")
+    seqs, B = _sequences(meta)
+    y = _out(out, T, C, act_dtype, u)
+    _check(lib().oxb_selective_scan(*at_u, *at_dt, *at_z, *at_b, *at_c, a.data_ptr(), _p(d), _p(dt_bias), *seqs, *_kept(state, "state"),
+                                    y.data_ptr(), y.stride(0), DT[act_dtype], B, T, C, N, meta.max_query_len, _stream()), "oxb_selective_scan")
     return y
