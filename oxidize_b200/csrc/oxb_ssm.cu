@@ -38,6 +38,7 @@ static int scan_go(ScanArgs a, cudaStream_t stream) {
 template <int L, int S>
 static int scan_step_go(ScanArgs a, cudaStream_t stream) {
   a.whole = S >= 4 && a.N == L * S && a.slot_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0;
+  a.wide = S >= 4 && a.N == L * S && scan_direct(a);
   constexpr int CH = 128 / L;
   oxb_launch(selective_step_kernel<L, S>, dim3((a.C + CH - 1) / CH, (a.s.B + L - 1) / L), dim3(128), 0, stream, a);
   OXB_CHECK_LAUNCH();

@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(ScanWide<NP>::CW) selective_scan_wide_kernel(c
 // Steps of one row per sequence.  grid (channels / (128 / L), B / L): a thread takes its states of L sequences through their tokens,
 // lane l prepares and ends one sequence's.  Bound by memory: the states are read and written once.
 template <int L, int S>
-__global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
+__global__ void __launch_bounds__(128, L * S <= 16 ? 10 : 1) selective_step_kernel(const ScanArgs a) {
   pdl_launch_dependents();
   pdl_wait();
   const int lane = threadIdx.x % L, c = blockIdx.x * (128 / L) + threadIdx.x / L, cc = min(c, a.C - 1);
@@ -684,20 +684,24 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
     const float dtj = __shfl_sync(0xffffffffu, dt, owner, L), duj = __shfl_sync(0xffffffffu, du, owner, L);
     acc[j] = 0.f;
     if (s < 0) continue;
-    uint32_t bb[S], cb[S];
-#pragma unroll
-    for (int i = 0; i < S; ++i) {
-      const int n = scan_state<S>(lane, i);
-      bb[i] = n < a.N ? ssm_bits(a.b, t, n) : 0u;
-      cb[i] = n < a.N ? ssm_bits(a.c, t, n) : 0u;
-    }
     float bv[S], cv[S];
+    if (S >= 4 && a.wide) {
+      scan_floats<S>(bv, reinterpret_cast<const float*>(a.b.p) + (size_t)t * a.b.ld, lane);
+      scan_floats<S>(cv, reinterpret_cast<const float*>(a.c.p) + (size_t)t * a.c.ld, lane);
+    } else {
+      uint32_t bb[S], cb[S];
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        const int n = scan_state<S>(lane, i);
+        bb[i] = n < a.N ? ssm_bits(a.b, t, n) : 0u;
+        cb[i] = n < a.N ? ssm_bits(a.c, t, n) : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < S; ++i) bv[i] = ssm_value(a.b, bb[i]), cv[i] = ssm_value(a.c, cb[i]);
+    }
     ScanState<S> h;
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      bv[i] = ssm_value(a.b, bb[i]), cv[i] = ssm_value(a.c, cb[i]);
-      h.h[i] = first[j][i], h.A2[i] = A2[i];
-    }
+    for (int i = 0; i < S; ++i) h.h[i] = first[j][i], h.A2[i] = A2[i];
     float e[S];
     h.decays(dtj, e);
     acc[j] = h.token(e, duj, bv, cv);
@@ -705,7 +709,7 @@ __global__ void __launch_bounds__(128) selective_step_kernel(const ScanArgs a) {
       float* to = a.state + s * a.slot_stride + (size_t)cc * a.N;
       if (S >= 4 && a.whole) {
 #pragma unroll
-        for (int i = 0; i + 3 < S; i += 4) *reinterpret_cast<float4*>(to + lane * S + i) = make_float4(h.h[i], h.h[i + 1], h.h[i + 2], h.h[i + 3]);
+        for (int i = 0; i + 3 < S; i += 4) __stcs(reinterpret_cast<float4*>(to + lane * S + i), make_float4(h.h[i], h.h[i + 1], h.h[i + 2], h.h[i + 3]));
       } else {
 #pragma unroll
         for (int i = 0; i < S; ++i)
