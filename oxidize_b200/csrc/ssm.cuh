@@ -139,7 +139,7 @@ __device__ __forceinline__ float ssm_softplus(float x) {
 }
 
 // The y-th longest of a step's sequences: long ones start first, so that short ones fill the gaps (9 of 331 to 1650 rows, 5120
-// channels: 440 us, 500 in their own order).  More than 32 even out by themselves and stay in their order.  Whole warps.
+// channels: 398 us, 501 in their own order).  More than 32 even out by themselves and stay in their order.  Whole warps.
 __device__ __forceinline__ int scan_sequence(const SsmStep& s, int y) {
   if (s.B > 32) return y;
   const int lane = threadIdx.x & 31, n = lane < s.B ? s.query_start[lane + 1] - s.query_start[lane] : -1;
@@ -297,10 +297,14 @@ struct ScanTile {
 // registers (as they are stored: a conversion would wait for its load) a tile ahead of their use, makes its tokens' steps, hands them
 // to the other lanes of the channel, and ends the tokens whose sums it gets.
 //
-// Alone on its quarter of an SM a warp takes as long as its instructions' latencies: 58 ns a token of 16 states with L = 8, 38 with 16.
-// With more warps it is bound by what shared memory can put into registers, 32 values a clock and SM: the step and b and c for every
-// lane of every channel, some 3 clocks per token and channel, against 1.2 for the 19 special functions (16 decays, the step's, two
-// for the gate).
+// Alone on its quarter of an SM a warp takes as long as its instructions' latencies: 58 ns a token of 16 states with L = 8, 30 with 16
+// (2048 rows of 1536 channels 104 us, of 256 channels 62).  With more warps it is bound by what shared memory can put into registers, 32
+// values a clock and SM: the step and b and c for every lane of every channel, some 3 clocks per token and channel, against 1.2 for the
+// 19 special functions (16 decays, the step's, two for the gate).
+//
+// Parts of a sequence beside one another (each one's end from zeros, joined, and then again from its first states) were measured as well:
+// 70 us for 2048 rows of 1536 channels, but from 512 rows or 5120 channels on the other side of it nothing (27 for 28, 194 for 184),
+// and results that depend on how a sequence is portioned.
 template <int L, int S, typename TU, typename TZ>
 __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
   using Tile = ScanTile<L, S>;
@@ -499,6 +503,10 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
 // The same with a lane to a channel and all of its states in registers, where there are channels enough to fill the SMs so: nothing is
 // handed from lane to lane, u, dt, z and y are whole lines of memory, and b and c come from shared memory to all lanes at once.
 // grid (channels / CW, B), CW threads; SB tokens of b and c at a time, TT of the rest.
+//
+// Bound by its instructions: 174 of them for a token and warp, which fill 64 % of the issue slots, and 20 special functions a channel (the
+// 16 decays among them), 56 % of that unit's; the states and the tokens in flight take the registers of the warps that would hide the rest.  9 sequences
+// of 331 to 1650 rows, 5120 channels: 398 us where the special functions alone take 189 and memory 60.
 template <int NP>
 struct ScanWide {
   static constexpr int CW = 32, SB = 32, TT = 8, STAGES = 3;
@@ -636,7 +644,8 @@ __global__ void __launch_bounds__(ScanWide<NP>::CW) selective_scan_wide_kernel(c
 }
 
 // Steps of one row per sequence.  grid (channels / (128 / L), B / L): a thread takes its states of L sequences through their tokens,
-// lane l prepares and ends one sequence's.  Bound by memory: the states are read and written once.
+// lane l prepares and ends one sequence's.  Bound by memory: the states are read and written once (256 sequences of 5120 channels with
+// 16 states: 40.6 us, 4.5 TB/s; with nine blocks to an SM 43, with a group's loads ahead of the one before it, which takes registers, 49).
 template <int L, int S>
 __global__ void __launch_bounds__(128, L * S <= 16 ? 10 : 1) selective_step_kernel(const ScanArgs a) {
   pdl_launch_dependents();
