@@ -236,6 +236,8 @@ struct I8Args {
   __nv_bfloat16* y;
   const float *sx, *sw, *bias;
   int N, T, K, ld_y, wide;  // wide: rows of y start on 16-byte boundaries and hold whole groups of 8
+  int token_tiles;
+  int whole;  // RB = 2: tiles ahead of this one are whole, the others halves of 128 weight rows
 };
 
 // A sum with its token's and its row's scale.  Its two halves become float32 by their bits and are joined with one rounding: as the
@@ -257,7 +259,7 @@ __device__ __forceinline__ void int8_store_rows(const __nv_bfloat16* stage, int 
   }
 }
 
-// grid (weight tiles, splits, token tiles).  With splits the CTAs of a tile are a cluster along K: whole-number sums meet in
+// grid (tiles, splits).  RB = 2: the tiles of a last wave that fills less than half of the SMs come as halves.  With splits the CTAs of a tile are a cluster along K: whole-number sums meet in
 // distributed shared memory, each CTA ends its share of the tokens (in any order the same sum; RB = 1 only).
 template <int TN, int RB>
 __global__ void __launch_bounds__(I8_THREADS, 1)
@@ -272,8 +274,10 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   float* tok_scale = reinterpret_cast<float*>(smem + Cfg::STAGES * Cfg::STAGE_BYTES + 256);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, splits = gridDim.y;
   // token tiles innermost: a weight tile is fetched from HBM once
-  const int lin = blockIdx.z * gridDim.x + blockIdx.x, tile_n = lin / (int)gridDim.z, tile_t = lin % (int)gridDim.z;
-  const int n0 = tile_n * (RB * I8_BM), t0 = tile_t * TN, kbs = (a.K + I8_BK - 1) / I8_BK;
+  int tile = blockIdx.x, half = 0, rb = RB;
+  if (RB == 2 && tile >= a.whole) half = (tile - a.whole) & 1, tile = a.whole + (tile - a.whole) / 2, rb = 1;
+  const int tile_n = tile / a.token_tiles, tile_t = tile % a.token_tiles;
+  const int n0 = (tile_n * RB + half) * I8_BM, t0 = tile_t * TN, kbs = (a.K + I8_BK - 1) / I8_BK;
   const int kb0 = (int)((long long)blockIdx.y * kbs / splits), nkb = (int)((long long)(blockIdx.y + 1) * kbs / splits) - kb0;
   if (threadIdx.x == 0) {
     for (int i = 0; i < Cfg::STAGES; ++i) {
@@ -300,16 +304,17 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     auto load_w = [&](int i, int st) {
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
+        if (r >= rb) break;
         uint8_t* to = smem + st * Cfg::STAGE_BYTES + r * (I8_BM * I8_BK);
         // (weights that one token tile reads need not stay in L2)
-        if (TN <= 128 && gridDim.z == 1) tma_load_2d_hint(to, &tmW, &full[st], (kb0 + i) * I8_BK, n0 + r * I8_BM, once);
+        if (TN <= 128 && a.token_tiles == 1) tma_load_2d_hint(to, &tmW, &full[st], (kb0 + i) * I8_BK, n0 + r * I8_BM, once);
         else tma_load_2d(to, &tmW, &full[st], (kb0 + i) * I8_BK, n0 + r * I8_BM);
       }
     };
     auto load_x = [&](int i, int st) { tma_load_2d(smem + st * Cfg::STAGE_BYTES + Cfg::A_BYTES, &tmX, &full[st], (kb0 + i) * I8_BK, t0); };
     if (leader)  // weights are static: they need not wait for the tokens
       for (int i = 0; i < npre; ++i) {
-        mbar_expect_tx(&full[i], Cfg::STAGE_BYTES);
+        mbar_expect_tx(&full[i], rb * (I8_BM * I8_BK) + Cfg::B_BYTES);
         load_w(i, i);
       }
     pdl_wait();
@@ -320,7 +325,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     for (int i = npre; i < nkb; ++i) {
       if (!__all_sync(0xffffffffu, int8_wait(&empty[st], ph, abort_flag, OXB_TIMEOUT_TMA_EMPTY, blockIdx.x))) break;
       if (leader) {
-        mbar_expect_tx(&full[st], Cfg::STAGE_BYTES);
+        mbar_expect_tx(&full[st], rb * (I8_BM * I8_BK) + Cfg::B_BYTES);
         load_w(i, st);
         load_x(i, st);
       }
@@ -340,7 +345,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
         for (int k = 0; k < I8_BK / 32; ++k)  // 32 values = 32 bytes of the swizzle row: +2 in the (address >> 4) field
 #pragma unroll
           for (int r = 0; r < RB; ++r)
-            umma_i8(tmem + r * TN, ad + r * (I8_BM * I8_BK >> 4) + 2 * k, bd + 2 * k, umma_idesc_i8(I8_BM, TN), i > 0 || k > 0);
+            if (r < rb) umma_i8(tmem + r * TN, ad + r * (I8_BM * I8_BK >> 4) + 2 * k, bd + 2 * k, umma_idesc_i8(I8_BM, TN), i > 0 || k > 0);
         umma_commit(&empty[st]);
       }
       if (++st == Cfg::STAGES) st = 0, ph ^= 1;
@@ -363,7 +368,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
     int* sums = reinterpret_cast<int*>(smem);
     const bool fine = !*abort_flag;
 #pragma unroll 1
-    for (int r = 0; r < RB; ++r) {
+    for (int r = 0; r < rb; ++r) {
       const int n1 = n0 + r * I8_BM, n = n1 + row;
       const float sw = n < a.N ? a.sw[n] : 0.f, b = n < a.N && a.bias != nullptr ? a.bias[n] : 0.f;
       if (fine) {
@@ -411,7 +416,7 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
       } else {
         asm volatile("bar.sync 1, 128;" ::: "memory");
         if (fine) int8_store_rows(stage, tvalid, t0, n1, a, threadIdx.x);
-        if (r + 1 < RB) asm volatile("bar.sync 1, 128;" ::: "memory");  // (the stage is written again)
+        if (r + 1 < rb) asm volatile("bar.sync 1, 128;" ::: "memory");  // (the stage is written again)
       }
     }
   }

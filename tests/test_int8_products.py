@@ -326,3 +326,20 @@ def test_few_tokens(T, k):
     q = weight(gen, 70, k, "cuda")
     x = torch.randn(T, k, generator=gen).bfloat16().cuda()
     check(x, q, None, ops.linear(x, LinearWeight([q])))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T,n,k", [(2053, 6001, 130), (2304, 6016, 1040), (4100, 9216, 64)])
+def test_last_waves(T, n, k):
+    """Some more tiles than SMs, or twice as many: the last ones come in halves, one of which may have no rows at all."""
+    from oxidize_b200.ops import cuda as C
+
+    gen = torch.Generator().manual_seed(n)
+    q = weight(gen, n, k, "cuda")
+    bias = torch.randn(n, generator=gen).cuda()
+    x = torch.randn(T, k, generator=gen).bfloat16().cuda()
+    out = torch.full((T, n + 8), 7.0, dtype=torch.bfloat16, device="cuda")
+    check(x, q, bias, ops.linear(x, LinearWeight([q], bias)))
+    ops.linear(x, LinearWeight([q], bias), out=out[:, :n])
+    check(x, q, bias, out[:, :n])
+    assert (out[:, n:] == 7).all() and C.status()[0] == 0
