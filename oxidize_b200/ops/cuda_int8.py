@@ -34,12 +34,19 @@ def linear(x: torch.Tensor, p, out_view: torch.Tensor, bias: Optional[torch.Tens
     T = x.shape[0]
     if x.shape[1] != k or k > MAX_K:
         raise ValueError(f"8-bit product of {x.shape[1]} values a token with a [{n}, {k}] matrix (at most {MAX_K} columns)")
-    if w.dtype != torch.int8 or w.stride(1) != 1 or w.stride(0) % 16 or w.data_ptr() % 16 or p.scales.dtype != torch.float32:
+    ld, one = w.stride()
+    if (w.dtype != torch.int8 or w.shape != (n, k) or one != 1 or ld % 16 or ld < k or w.data_ptr() % 16 or p.scales.dtype != torch.float32
+            or p.scales.shape != (n,) or not p.scales.is_contiguous()):
         raise ValueError("8-bit weights are int8 rows on 16-byte boundaries with float32 scales (quant.torch_quant.int8_rows)")
+    device = torch._C._cuda_getDevice()
+    if x.get_device() != device or w.get_device() != device or p.scales.get_device() != device or (bias is not None and bias.get_device() != device):
+        raise ValueError(f"an 8-bit product's tensors lie on the current device, cuda:{device}")
+    if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
+        bias = bias.float().contiguous()
     L = lib()
     made = rows is not None
     if not made and L.oxb_int8_needs_rows(T, k):
         rows = torch.empty(T * (-(-k // 16) * 16 + 4), dtype=torch.uint8, device=x.device)
-    _check(L.oxb_linear_int8(x.data_ptr(), T, k, _p(rows), int(made), w.data_ptr(), w.stride(0), p.scales.data_ptr(), _p(bias),
+    _check(L.oxb_linear_int8(x.data_ptr(), T, k, _p(rows), int(made), w.data_ptr(), ld, p.scales.data_ptr(), _p(bias),
                              out_view.data_ptr(), ld_out, n, _stream()), "oxb_linear_int8")
     return rows

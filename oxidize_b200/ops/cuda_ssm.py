@@ -26,6 +26,12 @@ def lib():
     return L
 
 
+def _elsewhere(here: int, **tensors: Optional[torch.Tensor]) -> ValueError:
+    """What the kernels are given lies on the current device, in whose stream they run."""
+    return ValueError(f"not on the current device, cuda:{here}: " + ", ".join(f"{k} on {v.device}" for k, v in tensors.items()
+                                                                             if v is not None and v.get_device() != here))
+
+
 def _rows(x: torch.Tensor, what: str):
     """(x with neighbouring columns, the three arguments that stand for it) in a type that the kernels read."""
     code = DT.get(x.dtype)
@@ -55,13 +61,16 @@ def _kept(v: torch.Tensor, what: str):
     return v.data_ptr(), step, n
 
 
-def _sequences(meta):
+def _sequences(meta, here: int):
     """Query starts, lengths with this step's rows, slots, and how many sequences there are."""
     starts, lens, slots = meta.query_start, meta.seq_lens, meta.state_slots
     n = lens.shape[0]
-    if starts.shape[0] <= n or slots.shape[0] < n or not starts.dtype == lens.dtype == slots.dtype == torch.int32:
-        raise ValueError(f"a step of {n} sequences has that many lengths and slots and a query start more, in int32, not {starts.dtype} "
+    if (starts.shape[0] <= n or slots.shape[0] < n or not starts.dtype == lens.dtype == slots.dtype == torch.int32
+            or not (starts.is_contiguous() and lens.is_contiguous() and slots.is_contiguous())):
+        raise ValueError(f"a step of {n} sequences has that many lengths and slots and a query start more, contiguous in int32, not {starts.dtype} "
                          f"{tuple(starts.shape)}, {lens.dtype} and {slots.dtype} {tuple(slots.shape)}")
+    if not starts.get_device() == lens.get_device() == slots.get_device() == here:
+        raise _elsewhere(here, query_start=starts, seq_lens=lens, state_slots=slots)
     return (starts.data_ptr(), lens.data_ptr(), slots.data_ptr()), n
 
 
@@ -77,9 +86,13 @@ def _out(out: Optional[torch.Tensor], T: int, C: int, dtype: torch.dtype, like: 
 
 def causal_conv(x, w, bias, meta, window, act, act_dtype, out=None):
     T, C = x.shape
+    here = torch._C._cuda_getDevice()
+    if not (x.get_device() == w.get_device() == window.get_device() == here and (bias is None or bias.get_device() == here)
+            and (out is None or out.get_device() == here)):
+        raise _elsewhere(here, x=x, w=w, bias=bias, window=window, out=out)
     x, at_x = _rows(x, "x")
     w, bias = _floats(w, "w"), _floats(bias, "bias")
-    seqs, B = _sequences(meta)
+    seqs, B = _sequences(meta, here)
     y = _out(out, T, C, act_dtype, x)
     _check(lib().oxb_causal_conv(*at_x, w.data_ptr(), _p(bias), *seqs, *_kept(window, "window"), y.data_ptr(), y.stride(0), DT[act_dtype], B, T, C,
                                  w.shape[1], act == "silu", meta.max_query_len, _stream()), "oxb_causal_conv")
@@ -91,12 +104,17 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype, out=No
     N = a.shape[1]
     if not 1 <= N <= MAX_STATES:
         raise ValueError(f"the scan takes 1 to {MAX_STATES} states, not {N}")
+    here = torch._C._cuda_getDevice()
+    if not (u.get_device() == dt.get_device() == a.get_device() == b.get_device() == c.get_device() == state.get_device() == here
+            and (z is None or z.get_device() == here) and (d is None or d.get_device() == here) and (dt_bias is None or dt_bias.get_device() == here)
+            and (out is None or out.get_device() == here)):
+        raise _elsewhere(here, u=u, dt=dt, a=a, b=b, c=c, d=d, z=z, dt_bias=dt_bias, state=state, out=out)
     if u.dtype != dt.dtype and u.dtype in DT and dt.dtype in DT:  # (the kernels read them as one type)
         u, dt = u.float(), dt.float()
     (u, at_u), (dt, at_dt), (b, at_b), (c, at_c) = _rows(u, "u"), _rows(dt, "dt"), _rows(b, "b"), _rows(c, "c")
     z, at_z = (None, (None, 0, 0)) if z is None else _rows(z, "z")
     a, d, dt_bias = _floats(a, "a"), _floats(d, "d"), _floats(dt_bias, "dt_bias")
-    seqs, B = _sequences(meta)
+    seqs, B = _sequences(meta, here)
     y = _out(out, T, C, act_dtype, u)
     _check(lib().oxb_selective_scan(*at_u, *at_dt, *at_z, *at_b, *at_c, a.data_ptr(), _p(d), _p(dt_bias), *seqs, *_kept(state, "state"),
                                     y.data_ptr(), y.stride(0), DT[act_dtype], B, T, C, N, meta.max_query_len, _stream()), "oxb_selective_scan")

@@ -343,3 +343,19 @@ def test_last_waves(T, n, k):
     ops.linear(x, LinearWeight([q], bias), out=out[:, :n])
     check(x, q, bias, out[:, :n])
     assert (out[:, n:] == 7).all() and C.status()[0] == 0
+
+
+@pytest.mark.gpu
+def test_what_lies_elsewhere_or_is_too_short_is_refused():
+    """Before anything is launched; a bias of another type is converted."""
+    gen = torch.Generator().manual_seed(10)
+    q, x = weight(gen, 40, 64, "cuda"), torch.randn(3, 64, generator=gen).bfloat16().cuda()
+    for bad in (QTensor("I8", q.data.cpu(), q.shape, q.scales), QTensor("I8", q.data, q.shape, q.scales.cpu()),
+                QTensor("I8", q.data, q.shape, q.scales[:39]), QTensor("I8", q.data[:39], q.shape, q.scales),
+                QTensor("I8", q.data, q.shape, q.scales[:1].expand(40))):
+        with pytest.raises(ValueError):
+            ops.linear(x, LinearWeight([bad]))
+    with pytest.raises(ValueError):
+        ops.linear(x, LinearWeight([q], torch.zeros(40)))
+    bias = torch.randn(40, generator=gen).bfloat16().cuda()
+    check(x, q, bias, ops.linear(x, LinearWeight([q], bias)))

@@ -378,6 +378,30 @@ def test_what_the_kernels_do_not_read_is_refused(call, change):
         call("cuda", **change)
 
 
+def _meta(**change):
+    def f(v):
+        for k, g in change.items():
+            setattr(v["meta"], k, g(getattr(v["meta"], k)))
+        return v["meta"]
+
+    return f
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("call,names", [(_scan_call, ("dt", "a", "b", "c", "d", "z", "dt_bias", "state")), (_conv_call, ("w", "bias", "window"))])
+def test_what_lies_elsewhere_or_is_too_short_is_refused(call, names):
+    """Before anything is launched: tensors of the host, metadata of other types or for fewer sequences."""
+    for name in names:
+        with pytest.raises(ValueError):
+            call("cuda", **{name: lambda v: v[name].cpu()})
+    with pytest.raises(ValueError):
+        call("cuda", out=lambda v: torch.zeros(4, 8))
+    for change in (dict(query_start=lambda q: q.cpu()), dict(seq_lens=lambda q: q.long()), dict(state_slots=lambda q: q[:0]),
+                   dict(query_start=lambda q: q[:1]), dict(query_start=lambda q: torch.stack([q, q], 1)[:, 0])):
+        with pytest.raises(ValueError):
+            call("cuda", meta=_meta(**change))
+
+
 # ------------------------------------------------------------------------------------------------- graphs and streams
 @pytest.mark.gpu
 @pytest.mark.parametrize("lens", [[1] * 5, [6, 1, 30]])
