@@ -48,7 +48,7 @@ __device__ __forceinline__ void conv_store(T* p, const float* v) {
 // The rows of a sequence that read its ring (the first K - 1) all belong to the tile of its first row, wherever the tile ends: the
 // thread that reads a ring is then also the one that writes it, afterwards.
 //
-// Bound by memory: a row is read and written once, but for the K - 1 rows ahead of a tile (L2 has them); its instructions fill 60 % of
+// Bound by memory: a row is read and written once, but for the K - 1 rows ahead of a tile (L2 has them); its instructions fill 45 % of
 // the issue slots, half of them silu's.  What counts are warps and plain code for whole groups of rows: 7 prompts of 300 to 1900 rows,
 // 4096 channels, bf16 to float32 48 us, 4.4 TB/s (52 with five blocks to an SM and every row guarded, 55 with the next group's rows loaded
 // ahead, which costs registers).

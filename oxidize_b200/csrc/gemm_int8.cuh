@@ -220,7 +220,7 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_
 constexpr int I8_BM = 128, I8_BK = 128;  // weight rows of an MMA; values of a k-block (one 128-byte swizzle row)
 constexpr int I8_THREADS = 192;          // warps 0-3: epilogue, 4: TMA, 5: MMA (which owns the tensor memory)
 
-// A tile of 128 RB weight rows x TN tokens.  What L2 can feed all SMs bounds many tokens (128 x 256: 48 KB per 512 clocks of products on
+// A tile of 128 RB weight rows x TN tokens.  What comes from L2 to all SMs bounds many tokens (128 x 256: 48 KB per 512 clocks of products on
 // every SM, 27 TB/s; some 11 come), so those take tiles of 256 x 256, which fill the tensor memory with their two accumulators: a
 // third less per product (8192 tokens of 8192 x 8192: 445 to 474 us, 2.3 to 2.5 P operations a second; 575 with 128 x 256).
 template <int TN, int RB>

@@ -505,7 +505,7 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
 // grid (channels / CW, B), CW threads; SB tokens of b and c at a time, TT of the rest.
 //
 // Bound by its instructions: 174 of them for a token and warp, which fill 64 % of the issue slots, and 20 special functions a channel (the
-// 16 decays among them), 56 % of that unit's; the states and the tokens in flight take the registers of the warps that would hide the rest.  9 sequences
+// 16 decays among them), 56 % of that unit's; 248 registers leave two warps to a scheduler (with 168, three, 404 us).  9 sequences
 // of 331 to 1650 rows, 5120 channels: 398 us where the special functions alone take 189 and memory 60.
 template <int NP>
 struct ScanWide {
