@@ -359,3 +359,19 @@ def test_what_lies_elsewhere_or_is_too_short_is_refused():
         ops.linear(x, LinearWeight([q], torch.zeros(40)))
     bias = torch.randn(40, generator=gen).bfloat16().cuda()
     check(x, q, bias, ops.linear(x, LinearWeight([q], bias)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [2, 20, 50, 65, 100, 128])
+@pytest.mark.parametrize("n,k", [(300, 4096), (100, 9000), (1025, 7300), (2600, 2100)])
+def test_sums_in_shares(T, n, k):
+    """Few weight tiles and long rows: several blocks share a tile's sums, each ends some of its tokens."""
+    from oxidize_b200.ops import cuda as C
+
+    gen = torch.Generator().manual_seed(T * n)
+    q = weight(gen, n, k, "cuda")
+    bias = torch.randn(n, generator=gen).cuda()
+    x = torch.randn(T, k, generator=gen).bfloat16().cuda()
+    y = ops.linear(x, LinearWeight([q], bias))
+    check(x, q, bias, y)
+    assert torch.equal(ops.linear(x, LinearWeight([q], bias)), y) and C.status()[0] == 0
