@@ -17,7 +17,7 @@ inline bool ssm_dtype(int d) { return d == 0 || d == 2; }
 // Rows and slots of a step's sequences.
 struct SsmStep {
   const int* query_start;  // [B + 1]
-  const int* seq_lens;     // [B], with this step's rows
+  const int* seq_lens;     // [B], with this step's rows (a smaller one is reported, and the sequence has no slot then)
   const int* slots;        // [B], < 0: none (rows of zeros come out)
   int B, T, num_slots;
 };
@@ -96,6 +96,10 @@ __device__ __forceinline__ SsmSeq ssm_seq(const SsmStep& s, int b, bool report) 
   q.pos0 = s.seq_lens[b] - (q.t1 - q.t0);
   if (q.slot >= s.num_slots) {
     if (report) oxb_report(OXB_BAD_SLOT, q.slot);
+    q.slot = -1;
+  }
+  if (q.slot >= 0 && q.pos0 < 0 && q.t1 > q.t0) {  // (rows of negative positions would lie ahead of the ring)
+    if (report) oxb_report(OXB_BAD_ARGUMENT, s.seq_lens[b]);
     q.slot = -1;
   }
   return q;

@@ -236,7 +236,9 @@ def causal_conv(x, w, bias, meta, window, act="silu", act_dtype=torch.float32, o
     + bias[c]) in ``act_dtype``.  x [T, C] (bfloat16 or float32, possibly columns of a wider projection), w [C, taps] and bias [C]
     float32, ``act`` "silu" or "none".  ``window`` [slots, taps, C] float32 is the ring of every sequence's last inputs (position p's
     row is row p % taps) and is updated; ``meta`` gives query_start, seq_lens, state_slots (no slot twice) and max_query_len.  Nothing
-    comes before position 0; rows of a sequence without a slot become zeros, rows behind the last sequence are left as they are."""
+    comes before position 0; rows of a sequence without a slot become zeros, rows behind the last sequence are left as they are.  A slot
+    past the store, or a length below the sequence's rows, is an error on the CPU; the device takes it for no slot and reports it in
+    its status word."""
     _check_recurrent(meta, window, "window")
     T, C = x.shape
     taps = w.shape[1]

@@ -510,6 +510,12 @@ def add_normed(res: torch.Tensor, y, w: torch.Tensor, groups: int, eps: float, a
     return x, None if act_dtype is None else x.to(act_dtype)
 
 
+def _first_position(length: int, rows: int) -> int:
+    if length < rows:
+        raise ValueError(f"a sequence of length {length} cannot have {rows} rows in this step")
+    return length - rows
+
+
 def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], meta, window: torch.Tensor, act: str,
                 act_dtype: torch.dtype) -> torch.Tensor:
     """Short depthwise convolution over each sequence's rows, act(sum_i w[c, i] x[t - (taps - 1) + i, c] + bias[c]): x [T, C],
@@ -524,7 +530,7 @@ def causal_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor], 
         m, ring = t1 - t0, window[slots[b]]
         if slots[b] < 0 or m == 0:
             continue
-        pos0 = lens[b] - m
+        pos0 = _first_position(lens[b], m)
         past = torch.stack([ring[p % n] if p >= 0 else torch.zeros_like(ring[0]) for p in range(pos0 - n + 1, pos0)] or [ring[0]])
         rows = torch.cat([past[: n - 1], xf[t0:t1]])
         conv = sum(wf[:, j] * rows[j : j + m] for j in range(n))
@@ -550,7 +556,7 @@ def selective_scan(u: torch.Tensor, dt: torch.Tensor, a: torch.Tensor, b: torch.
         t0, t1 = qs[i], qs[i + 1]
         if slots[i] < 0 or t1 == t0:
             continue
-        h = torch.zeros_like(state[slots[i]]) if lens[i] == t1 - t0 else state[slots[i]]
+        h = torch.zeros_like(state[slots[i]]) if _first_position(lens[i], t1 - t0) == 0 else state[slots[i]]
         for t in range(t0, t1):
             h = torch.exp(af * step[t][:, None]) * h + (step[t] * uf[t])[:, None] * bf[t][None, :]
             y[t] = h @ cf[t] + (0 if d is None else d.float() * uf[t])

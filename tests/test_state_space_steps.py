@@ -1,0 +1,40 @@
+"""Steps of state-space layers that the tests of ``test_state_space.py`` do not make: metadata that contradicts itself, kernels that
+only wide steps reach, values that are not finite, outputs over inputs.  Statements in 64 bits, bounds and tolerances are those."""
+import pytest
+import torch
+
+from oxidize_b200 import ops
+from test_state_space import DEVICES, scan_inputs, step
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("taps", [3, 4, 6])
+@pytest.mark.parametrize("lens", [[1, 1, 1], [3, 5, 2]])
+def test_lengths_below_the_rows_of_a_step(lens, taps, device):
+    """A length that leaves a sequence's rows before position 0: refused on the CPU; on the device its rows become zeros, nothing is
+    written for it, the status word has the length, and its neighbours are as without it."""
+    gen = torch.Generator().manual_seed(31)
+    C, N, T = 40, 16, sum(lens)
+    v = scan_inputs(gen, T, C, N, "f32", "f32", "f32", "f32", True, True, True, 0, device)
+    w = torch.randn(C, taps, generator=gen).to(device)
+    # (slot 1 in the middle of the store: what lies ahead of its ring is slot 0's)
+    window, state = torch.randn(3, taps, C, generator=gen).to(device), torch.randn(3, C, N, generator=gen).to(device)
+    bad, none = step(lens, device, slots=(0, 1, 2)), step(lens, device, slots=(0, -1, 2))
+    bad.seq_lens[1] = lens[1] - 1
+    if device == "cpu":
+        with pytest.raises(ValueError, match="length"):
+            ops.causal_conv(v["u"], w, None, bad, window)
+        with pytest.raises(ValueError, match="length"):
+            ops.selective_scan(**v, meta=bad, state=state)
+        return
+    from oxidize_b200.ops import cuda as K
+
+    window1, state1 = window.clone(), state.clone()
+    K.status()
+    y = ops.causal_conv(v["u"], w, None, bad, window)
+    assert K.status()[:2] == (8, lens[1] - 1)
+    s = ops.selective_scan(**v, meta=bad, state=state)
+    assert K.status()[:2] == (8, lens[1] - 1)
+    y1, s1 = ops.causal_conv(v["u"], w, None, none, window1), ops.selective_scan(**v, meta=none, state=state1)
+    assert K.status()[0] == 0
+    assert torch.equal(y, y1) and torch.equal(s, s1) and torch.equal(window, window1) and torch.equal(state, state1)
