@@ -13,6 +13,7 @@ from .cuda import _check, _p, _stream
 _declared = False
 DT = {torch.float32: 0, torch.bfloat16: 2}
 MAX_STATES = 128
+MAX_STRIDE = 2 ** 31 - 1  # values from row to row: a 32-bit number for the kernels (offsets of rows are 64-bit ones)
 
 
 def lib():
@@ -38,7 +39,7 @@ def _rows(x: torch.Tensor, what: str):
     if code is None:
         raise ValueError(f"{what} is float32 or bfloat16, not {x.dtype}")
     ld, one = x.stride()
-    if one != 1 and x.shape[1] != 1:
+    if (one != 1 and x.shape[1] != 1) or (ld > MAX_STRIDE and x.shape[0] > 1):
         x = x.contiguous()
         ld = x.stride(0)
     return x, (x.data_ptr(), ld, code)
@@ -81,6 +82,8 @@ def _out(out: Optional[torch.Tensor], T: int, C: int, dtype: torch.dtype, like: 
         return like.new_empty((T, C), dtype=dtype)
     if out.shape != (T, C) or out.dtype != dtype or (out.stride(1) != 1 and C > 1):
         raise ValueError(f"out is [{T}, {C}] in {dtype} with neighbouring columns, not {tuple(out.shape)} in {out.dtype}")
+    if out.stride(0) > MAX_STRIDE and T > 1:
+        raise ValueError(f"rows of out are at most {MAX_STRIDE} values apart, not {out.stride(0)}")
     return out
 
 

@@ -38,3 +38,22 @@ def test_lengths_below_the_rows_of_a_step(lens, taps, device):
     y1, s1 = ops.causal_conv(v["u"], w, None, none, window1), ops.selective_scan(**v, meta=none, state=state1)
     assert K.status()[0] == 0
     assert torch.equal(y, y1) and torch.equal(s, s1) and torch.equal(window, window1) and torch.equal(state, state1)
+
+
+@pytest.mark.parametrize("apart", [2 ** 31 - 1, 2 ** 31, 2 ** 32 + 8])
+def test_rows_far_apart(apart):
+    """The kernels take the distance of rows as a 32-bit number: rows further apart are copied, such an output is refused; one row
+    alone has no next one.  (Of the bindings, which launch nothing here: tensors without storage.)"""
+    from oxidize_b200.ops import cuda_ssm
+
+    far = torch.empty_strided((2, 8), (apart, 1), device="meta")
+    x, (_, ld, code) = cuda_ssm._rows(far, "x")
+    assert x.shape == (2, 8) and code == 0 and ld == (apart if apart < 2 ** 31 else 8)
+    one, _ = cuda_ssm._rows(far[:1], "x")
+    assert one.stride() == (apart, 1)
+    if apart < 2 ** 31:
+        assert cuda_ssm._out(far, 2, 8, torch.float32, far) is far
+    else:
+        with pytest.raises(ValueError, match="apart"):
+            cuda_ssm._out(far, 2, 8, torch.float32, far)
+    assert cuda_ssm._out(far[:1], 1, 8, torch.float32, far) is not None
