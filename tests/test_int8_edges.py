@@ -1,0 +1,51 @@
+"""Calls of products on 8-bit integers that ``test_int8_products.py`` does not make.  Its statement in 64 bits and its bounds."""
+import pytest
+import torch
+
+from oxidize_b200 import ops
+from oxidize_b200.models.weights import LinearWeight, QTensor
+from oxidize_b200.quant import torch_quant
+from test_int8_products import check, weight
+
+
+def far(n, k, apart, dtype):
+    return torch.empty_strided((n, k), (apart, 1), dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("change", [
+    dict(bias=torch.zeros(39)), dict(bias=torch.zeros(40, 1)),  # shorter than the outputs; of two dimensions
+    dict(out=torch.zeros(3, 40)), dict(out=torch.zeros(2, 40, dtype=torch.bfloat16)),  # of another type; too few rows
+    dict(out=torch.zeros(3, 39, dtype=torch.bfloat16)), dict(out=torch.zeros(40, 3, dtype=torch.bfloat16).t()),  # too few columns; in columns
+    dict(out=torch.zeros(1, 40, dtype=torch.bfloat16).expand(3, 40)),  # every row the same
+    dict(out=far(3, 40, 2 ** 31, torch.bfloat16)), dict(codes=far(40, 64, 2 ** 31, torch.int8))])  # rows too far apart
+def test_what_does_not_fit_is_refused_ahead_of_the_launch(change, monkeypatch):
+    """On tensors of the host, which pass for the current device's here, and without a library to launch anything."""
+    from oxidize_b200.ops import cuda_int8
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1)
+
+    def launch():
+        raise AssertionError("launched")
+
+    monkeypatch.setattr(cuda_int8, "lib", launch)
+    x = torch.zeros(3, 64, dtype=torch.bfloat16)
+    codes = change.get("codes", torch_quant.int8_rows(torch.zeros(40, 64, dtype=torch.int8)))
+    q = QTensor("I8", codes, (40, 64), torch.ones(40))
+    out = change.get("out", torch.zeros(3, 40, dtype=torch.bfloat16))
+    with pytest.raises(ValueError):
+        cuda_int8.linear(x, q, out, change.get("bias"), out.stride(0))
+    with pytest.raises(AssertionError, match="launched"):
+        cuda_int8.linear(x, QTensor("I8", torch.zeros(40, 64, dtype=torch.int8), (40, 64), torch.ones(40)), torch.zeros(4, 48, dtype=torch.bfloat16),
+                         torch.zeros(41), 48)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 3, 200])
+def test_longer_biases_and_larger_outputs(T):
+    """Their first values: what lies behind stays as it was."""
+    gen = torch.Generator().manual_seed(41)
+    q, x = weight(gen, 40, 64, "cuda"), torch.randn(T, 64, generator=gen).bfloat16().cuda()
+    bias, out = torch.randn(50, generator=gen).cuda(), torch.full((T + 2, 56), 7.0, dtype=torch.bfloat16, device="cuda")
+    ops.linear(x, LinearWeight([q], bias), out=out)
+    check(x, q, bias[:40], out[:T, :40])
+    assert (out[T:] == 7).all() and (out[:, 40:] == 7).all()
