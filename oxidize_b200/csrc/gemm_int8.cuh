@@ -334,6 +334,9 @@ gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant_
   } else if (warp == 5) {
     const bool leader = elect_one();
     const uint32_t base = smem_u32(smem);
+    // No operands come before the tokens do: ahead of this the bound on waits would count what earlier kernels still have to do (an
+    // all-reduce may wait for its peers longer than that).
+    pdl_wait();
     int st = 0;
     uint32_t ph = 0;
     for (int i = 0; i < nkb; ++i) {

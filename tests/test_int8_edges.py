@@ -49,3 +49,32 @@ def test_longer_biases_and_larger_outputs(T):
     ops.linear(x, LinearWeight([q], bias), out=out)
     check(x, q, bias[:40], out[:T, :40])
     assert (out[T:] == 7).all() and (out[:, 40:] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [2, 300])
+def test_behind_a_kernel_that_runs_for_seconds(T):
+    """The product is resident while a kernel ahead of it, which let its dependents start, still runs for longer than a wait's bound of a
+    second: the time of that kernel does not count."""
+    from types import SimpleNamespace
+
+    from oxidize_b200.ops import cuda as C
+
+    gen = torch.Generator().manual_seed(43)
+    q, x = weight(gen, 200, 256, "cuda"), torch.randn(T, 256, generator=gen).bfloat16().cuda()
+    want = ops.linear(x, LinearWeight([q]))
+    # a convolution of one channel and very many taps: one thread's work, some seconds of it
+    taps = 12_000_000
+    w, window, row = torch.zeros(1, taps, device="cuda"), torch.zeros(1, taps, 1, device="cuda"), torch.zeros(1, 1, device="cuda")
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    meta = SimpleNamespace(query_start=i32(0, 1), seq_lens=i32(taps + 1), state_slots=i32(0), max_query_len=1)
+    torch.cuda.synchronize()
+    C.status()
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    ops.causal_conv(row, w, None, meta, window, act="none")
+    y = ops.linear(x, LinearWeight([q]))
+    end.record()
+    torch.cuda.synchronize()
+    assert begin.elapsed_time(end) > 1500
+    assert C.status()[0] == 0 and torch.equal(y, want)
