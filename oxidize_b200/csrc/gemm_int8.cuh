@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(256) gemv_int8_kernel(const __nv_bfloat16* __r
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
     if (lane == 0 && row0 + r < N)
-      y[row0 + r] = __float2bfloat16(__int2float_rn(a) * scale * sw[row0 + r] + (bias != nullptr ? bias[row0 + r] : 0.f));
+      y[row0 + r] = __float2bfloat16(__int2float_rn(a) * sw[row0 + r] * scale + (bias != nullptr ? bias[row0 + r] : 0.f));
   }
 }
 
@@ -240,11 +240,12 @@ struct I8Args {
   int whole;  // RB = 2: tiles ahead of this one are whole, the others halves of 128 weight rows
 };
 
-// A sum with its token's and its row's scale.  Its two halves become float32 by their bits and are joined with one rounding: as the
-// conversion instruction, which is one of the slow special function unit's.
+// A sum with its row's and its token's scale, in this order: a large token's scale alone would take the sum past float32's range.  The
+// sum's two halves become float32 by their bits and are joined with one rounding: as the conversion instruction, which is one of the slow
+// special function unit's.
 __device__ __forceinline__ float int8_result(int sum, float sx, float sw, float b) {
   const float hi = __uint_as_float(0x4B400000u + (uint32_t)(sum >> 16)) - 12582912.f, lo = __uint_as_float(0x4B000000u | ((uint32_t)sum & 0xFFFF)) - 8388608.f;
-  return fmaf(hi, 65536.f, lo) * sx * sw + b;
+  return fmaf(hi, 65536.f, lo) * sw * sx + b;
 }
 
 // [token][128 rows] of bf16 in shared memory to y's rows, by 128 threads

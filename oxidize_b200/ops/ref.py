@@ -52,7 +52,7 @@ def linear_int8(x: torch.Tensor, w, bias: Optional[torch.Tensor] = None) -> torc
     """x @ W^T on 8-bit integers (``w``: codes [out, in] with a scale per row; ``x`` gets one per token): whole-number sums, scaled
     and rounded once."""
     codes, scale = quantize_tokens(x)
-    y = (codes @ w.data.double().t()).float() * scale * w.scales
+    y = (codes @ w.data.double().t()).float() * w.scales * scale  # (the token's scale may be large: last)
     if bias is not None:
         y = y + bias.float()
     return y.to(x.dtype)

@@ -3,9 +3,9 @@ import pytest
 import torch
 
 from oxidize_b200 import ops
-from oxidize_b200.models.weights import LinearWeight, QTensor
+from oxidize_b200.models.weights import LinearWeight, QTensor, qtensor_from_dense
 from oxidize_b200.quant import torch_quant
-from test_int8_products import check, weight
+from test_int8_products import DEVICES, check, tokens, weight
 
 
 def far(n, k, apart, dtype):
@@ -78,3 +78,15 @@ def test_behind_a_kernel_that_runs_for_seconds(T):
     torch.cuda.synchronize()
     assert begin.elapsed_time(end) > 1500
     assert C.status()[0] == 0 and torch.equal(y, want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("T", [1, 3, 40, 300])
+def test_large_tokens(T, device):
+    """Tokens around 1e35, whose sums times their scales alone would leave float32's range, with weights that bring them back."""
+    gen = torch.Generator().manual_seed(44)
+    x = tokens(torch.randn(T, 4096, generator=gen) * 2e35, device)
+    q = qtensor_from_dense(torch.randn(200, 4096, generator=gen) * 0.02, "I8", device)
+    y = ops.linear(x, LinearWeight([q]))
+    assert torch.isfinite(y).all() and y.abs().max() > 1e35
+    check(x, q, None, y)
