@@ -364,7 +364,8 @@ class Transformer:
         self._ssm_clock += 1
         qs, first, pos0 = meta.query_start.tolist(), meta.block_tables[:, 0].tolist(), meta.positions.tolist()
         slots = [self._ssm_slot(kv, first[b], pos0[qs[b]]) if qs[b + 1] > qs[b] else -1 for b in range(len(qs) - 1)]
-        step = replace(meta, state_slots=torch.tensor(slots, dtype=torch.int32, device=self.device))
+        # (an ``extra`` of its own: the step lies in meta's, and would otherwise hold itself, and its tensors, until a cycle is collected)
+        step = replace(meta, state_slots=torch.tensor(slots, dtype=torch.int32, device=self.device), extra={})
         meta.extra["ssm_step"] = step
         return step
 

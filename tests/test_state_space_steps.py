@@ -57,3 +57,28 @@ def test_rows_far_apart(apart):
         with pytest.raises(ValueError, match="apart"):
             cuda_ssm._out(far, 2, 8, torch.float32, far)
     assert cuda_ssm._out(far[:1], 1, 8, torch.float32, far) is not None
+
+
+def test_steps_of_a_model_are_freed_with_their_last_name(tmp_path, monkeypatch):
+    """Without Python's collector of cycles: a step's tensors go when the step does."""
+    import gc
+    import weakref
+
+    from test_int8_products import _llm, _tiny_mamba
+
+    llm = _llm(_tiny_mamba(tmp_path), "cpu", "")
+    seen, slots_of = [], llm.model._ssm_step
+
+    def watched(meta, kv, first_layer):
+        out = slots_of(meta, kv, first_layer)
+        seen.extend((weakref.ref(meta), weakref.ref(out), weakref.ref(out.state_slots)))
+        return out
+
+    monkeypatch.setattr(llm.model, "_ssm_step", watched)
+    gc.collect()
+    gc.disable()
+    try:
+        llm.next_token_logits([[5, 9, 20], [31]])
+        assert len(seen) >= 6 and all(r() is None for r in seen)
+    finally:
+        gc.enable()
