@@ -381,8 +381,10 @@ class Transformer:
         # products on the decoded matrices) instead of going through the bf16 GEMM
         par = u @ m.x_proj.dense_cache().float().t()
         dt = par[:, :R] @ m.dt_proj.dense_cache().float().t()
-        y = ops.selective_scan(u, dt, m.a, par[:, R : R + N], par[:, R + N :], m.d, xz[:, di:], m.dt_bias, step,
-                               self._ssm_state[:, layer], act_dtype=x.dtype)
+        # (the kernel takes up to 128 states a channel; more run token by token from the host)
+        scan = ops.selective_scan if N <= ops.MAX_SCAN_STATES or not x.is_cuda else opref.selective_scan
+        y = scan(u, dt, m.a, par[:, R : R + N], par[:, R + N :], m.d, xz[:, di:], m.dt_bias, step,
+                 self._ssm_state[:, layer], act_dtype=x.dtype)
         return ops.linear(y, m.out_proj)
 
     def _gated_delta(self, lw: LayerWeights, layer: int, x: torch.Tensor, meta: BatchMeta, kv) -> torch.Tensor:

@@ -52,6 +52,9 @@ def _cuda_ssm():
     return _c
 
 
+MAX_SCAN_STATES = 128  # a channel's states that the device's selective scan takes
+
+
 class DepthStreams:
     """The embedding and the layers' results of a step, kept for the weighted sums that go on from layer to layer."""
 
@@ -260,7 +263,7 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype=torch.f
     columns of wider projections; z None: no gate); a [C, N], d [C], dt_bias [C] float32 (d, dt_bias None: zeros); ``state`` [slots, C,
     N] float32 is updated.  ``meta`` as for ``causal_conv``.  A sequence whose rows start at position 0 starts from nothing; rows of
     one without a slot become zeros, rows behind the last sequence are left as they are.  A sequence's result does not depend on
-    the portions that its rows come in, nor on its neighbours."""
+    the portions that its rows come in, nor on its neighbours.  On the device N is at most ``MAX_SCAN_STATES``."""
     _check_recurrent(meta, state, "state")
     T, C = u.shape
     N = a.shape[1]

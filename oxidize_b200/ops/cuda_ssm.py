@@ -7,12 +7,12 @@ from typing import Optional
 
 import torch
 
+from . import MAX_SCAN_STATES
 from . import cuda as opcuda
 from .cuda import _check, _p, _stream
 
 _declared = False
 DT = {torch.float32: 0, torch.bfloat16: 2}
-MAX_STATES = 128
 MAX_STRIDE = 2 ** 31 - 1  # values from row to row: a 32-bit number for the kernels (offsets of rows are 64-bit ones)
 
 
@@ -105,8 +105,8 @@ def causal_conv(x, w, bias, meta, window, act, act_dtype, out=None):
 def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype, out=None):
     T, C = u.shape
     N = a.shape[1]
-    if not 1 <= N <= MAX_STATES:
-        raise ValueError(f"the scan takes 1 to {MAX_STATES} states, not {N}")
+    if not 1 <= N <= MAX_SCAN_STATES:
+        raise ValueError(f"the scan takes 1 to {MAX_SCAN_STATES} states, not {N}")
     here = torch._C._cuda_getDevice()
     if not (u.get_device() == dt.get_device() == a.get_device() == b.get_device() == c.get_device() == state.get_device() == here
             and (z is None or z.get_device() == here) and (d is None or d.get_device() == here) and (dt_bias is None or dt_bias.get_device() == here)

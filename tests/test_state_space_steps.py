@@ -82,3 +82,29 @@ def test_steps_of_a_model_are_freed_with_their_last_name(tmp_path, monkeypatch):
         assert len(seen) >= 6 and all(r() is None for r in seen)
     finally:
         gc.enable()
+
+
+def _mamba_with_states(directory, states):
+    T = pytest.importorskip("transformers")
+    from oxidize_b200.formats.convert import convert_safetensors_to_gguf
+
+    torch.manual_seed(0)
+    model = T.MambaForCausalLM(T.MambaConfig(vocab_size=300, hidden_size=64, state_size=states, num_hidden_layers=2, conv_kernel=4, expand=2,
+                                             time_step_rank=4))
+    model.save_pretrained(str(directory / "hf"), safe_serialization=True)
+    return convert_safetensors_to_gguf(str(directory / "hf"), str(directory / "m.gguf"), "F32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("states", [128, 129, 200])
+def test_models_with_many_states(states, tmp_path):
+    """On either side of what the scan's kernel takes, against the CPU (the tolerance of the other engine tests: bfloat16 projections)."""
+    from test_int8_products import _far, _llm
+
+    path = _mamba_with_states(tmp_path, states)
+    cpu, gpu = _llm(path, "cpu", ""), _llm(path, "cuda", "")
+    prompts = [[5, 9, 20, 31, 200, 7], [17]]
+    for _ in range(2):
+        a, b = cpu.next_token_logits(prompts), gpu.next_token_logits(prompts)
+        assert _far(b, a) < 0.1
+        prompts = [p + [int(torch.as_tensor(a)[i].argmax())] for i, p in enumerate(prompts)]
