@@ -8,15 +8,15 @@ static bool scan_direct(const ScanArgs& a) {
          ((reinterpret_cast<uintptr_t>(a.b.p) | reinterpret_cast<uintptr_t>(a.c.p)) & 15) == 0;
 }
 
-template <int L, int S, typename TU, typename TZ>
+template <int L, int S, bool ALL, typename TU, typename TZ>
 static int scan_typed(const ScanArgs& a, cudaStream_t stream) {
   constexpr int CH = ScanTile<L, S>::CH;
-  return (int)oxb_launch(selective_scan_kernel<L, S, TU, TZ>, dim3((a.C + CH - 1) / CH, a.s.B), dim3(128), 0, stream, a);
+  return (int)oxb_launch(selective_scan_kernel<L, S, ALL, TU, TZ>, dim3((a.C + CH - 1) / CH, a.s.B), dim3(128), 0, stream, a);
 }
-template <int NP, typename TU, typename TZ>
+template <int NP, bool ALL, typename TU, typename TZ>
 static int scan_wide_typed(const ScanArgs& a, cudaStream_t stream) {
   constexpr int CW = ScanWide<NP>::CW;
-  return (int)oxb_launch(selective_scan_wide_kernel<NP, TU, TZ>, dim3((a.C + CW - 1) / CW, a.s.B), dim3(CW), 0, stream, a);
+  return (int)oxb_launch(selective_scan_wide_kernel<NP, ALL, TU, TZ>, dim3((a.C + CW - 1) / CW, a.s.B), dim3(CW), 0, stream, a);
 }
 // by the types of u, dt and of the gate
 #define SCAN_TYPES(F, ...)                                                                          \
@@ -30,7 +30,7 @@ static int scan_wide_typed(const ScanArgs& a, cudaStream_t stream) {
 template <int L, int S>
 static int scan_go(ScanArgs a, cudaStream_t stream) {
   a.wide = scan_direct(a);
-  const int e = SCAN_TYPES(scan_typed, L, S);
+  const int e = a.N == L * S ? SCAN_TYPES(scan_typed, L, S, true) : SCAN_TYPES(scan_typed, L, S, false);
   if (e != 0) return e;
   OXB_CHECK_LAUNCH();
   return 0;
@@ -40,14 +40,16 @@ static int scan_step_go(ScanArgs a, cudaStream_t stream) {
   a.whole = S >= 4 && a.N == L * S && a.slot_stride % 4 == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0;
   a.wide = S >= 4 && a.N == L * S && scan_direct(a);
   constexpr int CH = 128 / L;
-  oxb_launch(selective_step_kernel<L, S>, dim3((a.C + CH - 1) / CH, (a.s.B + L - 1) / L), dim3(128), 0, stream, a);
+  const dim3 grid((a.C + CH - 1) / CH, (a.s.B + L - 1) / L);
+  if (a.N == L * S) oxb_launch(selective_step_kernel<L, S, true>, grid, dim3(128), 0, stream, a);
+  else oxb_launch(selective_step_kernel<L, S, false>, grid, dim3(128), 0, stream, a);
   OXB_CHECK_LAUNCH();
   return 0;
 }
 template <int NP>
 static int scan_wide_go(ScanArgs a, cudaStream_t stream) {
   a.wide = scan_direct(a);
-  const int e = SCAN_TYPES(scan_wide_typed, NP);
+  const int e = a.N == NP ? SCAN_TYPES(scan_wide_typed, NP, true) : SCAN_TYPES(scan_wide_typed, NP, false);
   if (e != 0) return e;
   OXB_CHECK_LAUNCH();
   return 0;

@@ -204,7 +204,22 @@ struct ScanState {
       h[i] = fmaf(e[i], h[i], __fmul_rn(su, b[i]));
       p[i] = __fmul_rn(h[i], c[i]);
     }
-    // states that differ in bit 1, then 0, then 2 and so on (two states to a lane differ in bit 1)
+    return sum(p);
+  }
+  // The token's share once more, after a step that is not finite: it has turned the zeros past state N into NaN, which do not count and
+  // become zeros again.
+  __device__ __forceinline__ float without_rest(const float (&c)[S], int lane, int N) {
+    float p[S];
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+      const bool on = scan_state<S>(lane, i) < N;
+      p[i] = on ? __fmul_rn(h[i], c[i]) : 0.f;
+      if (!on) h[i] = 0.f;
+    }
+    return sum(p);
+  }
+  // states that differ in bit 1, then 0, then 2 and so on (two states to a lane differ in bit 1)
+  static __device__ __forceinline__ float sum(float (&p)[S]) {
     if constexpr (S >= 4) {
 #pragma unroll
       for (int i = 0; i < S; i += 4) p[i] = __fadd_rn(__fadd_rn(p[i], p[i + 2]), __fadd_rn(p[i + 1], p[i + 3]));
@@ -218,6 +233,9 @@ struct ScanState {
     return p[0];
   }
 };
+
+// Whether a step times its input is not finite
+__device__ __forceinline__ bool scan_strange(float su) { return !(fabsf(su) < __int_as_float(0x7F800000)); }
 
 // From each lane's shares of L tokens to the whole of one token: lanes that differ in one bit swap halves of what they hold, bit
 // after bit.  Lane l ends with token scan_turn(l).
@@ -294,6 +312,9 @@ struct ScanTile {
   float4 steps[4][2][TT / 2][32 / L];  // (s, s u) of two tokens; each warp's own, this tile's and the next one's
 };
 
+// ALL: there are NP states.  Otherwise those past N have to stay zeros whatever the steps are: one that is not finite takes its warp's tile
+// through the code that leaves them out.
+//
 // grid (channels / CH, B): CTA (i, b) takes CH channels of sequence b through its rows, a tile of tokens at a time; L lanes share a
 // channel.  For steps with few channels, all sequences' together.
 //
@@ -309,7 +330,7 @@ struct ScanTile {
 // Parts of a sequence beside one another (each one's end from zeros, joined, and then again from its first states) were measured as well:
 // 70 us for 2048 rows of 1536 channels, but from 512 rows or 5120 channels on the other side of it nothing (27 for 28, 194 for 184),
 // and results that depend on how a sequence is portioned.
-template <int L, int S, typename TU, typename TZ>
+template <int L, int S, bool ALL, typename TU, typename TZ>
 __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
   using Tile = ScanTile<L, S>;
   constexpr int NP = Tile::NP, G = Tile::G, TT = Tile::TT, STAGES = Tile::STAGES, PARTS = 2 * TT * NP / 128;
@@ -409,6 +430,15 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
       }
     }
   };
+  // Whether a warp's tile has steps that only the code for any step takes right
+  auto odd = [&](const float2 (&step)[G]) {
+    if constexpr (ALL) return false;
+    bool any = false;
+#pragma unroll
+    for (int g = 0; g < G; ++g) any |= scan_strange(step[g].y);
+    return __any_sync(0xffffffffu, any) != 0;
+  };
+  bool strange;
   scan_load<G, L>(U, a.u.ld, q.t0 + turn, last, pu);
   scan_load<G, L>(DT, a.dt.ld, q.t0 + turn, last, pd);
   {
@@ -418,6 +448,7 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
     float2 step[G];
     prepare(step);
     keep_steps(0, step);
+    strange = odd(step);
 #pragma unroll
     for (int g = 0; g < G; ++g) pu[g] = nu[g], pd[g] = nd[g], eu[g] = ez[g] = 0, y[g] = 0.f;
   }
@@ -437,7 +468,7 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
     const float *Bt = sm.bc[i % STAGES][0], *Ct = sm.bc[i % STAGES][1];
     const float4(*steps)[32 / L] = sm.steps[tid / 32][i & 1];
     const int n = q.t1 - q.t0 - i * TT;
-    if (n >= TT) {  // (all in one block of code, for the compiler to interleave)
+    if (n >= TT && !strange) {  // (all in one block of code, for the compiler to interleave)
       prepare(step);
       end(done);
       constexpr int P = S > 4 ? 2 : 4;  // tokens at a time: first all that does not depend on the token before
@@ -463,7 +494,7 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
         }
         sums[g] = scan_join<L, S>(acc, lane);
       }
-    } else {  // the sequence's last tokens
+    } else {  // the sequence's last tokens, or any steps
       prepare(step);
       end(done);
 #pragma unroll
@@ -480,6 +511,7 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
             const float2 st = reinterpret_cast<const float2*>(&steps[t / 2][wc])[t & 1];
             h.decays(st.x, e);
             acc[j] = h.token(e, st.y, bv, cv);
+            if (strange) acc[j] = h.without_rest(cv, lane, a.N);
           }
         }
         sums[g] = scan_join<L, S>(acc, lane);
@@ -487,6 +519,7 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
     }
     store(i - 1, done);
     keep_steps(i + 1, step);
+    strange = odd(step);
     if (i + 2 < tiles) keep_bc(i + 2);
 #pragma unroll
     for (int g = 0; g < G; ++g) pu[g] = nu[g], pd[g] = nd[g], eu[g] = fu[g], ez[g] = GATE ? fz[g] : 0, y[g] = sums[g];
@@ -515,7 +548,38 @@ template <int NP>
 struct ScanWide {
   static constexpr int CW = 32, SB = 32, TT = 8, STAGES = 3;
 };
-template <int NP, typename TU, typename TZ>
+// One channel of a sequence, from its start, token by token: where a step was not finite and there are states past N, which it turned into
+// NaN.  Only the state's end shows it: a look at every step cost up to 12 %.
+template <int NP>
+__device__ __forceinline__ void scan_channel(const ScanArgs& a, const SsmSeq& q, int c) {
+  float* state = a.state + q.slot * a.slot_stride + (size_t)c * a.N;
+  ScanState<NP> h;
+#pragma unroll
+  for (int n = 0; n < NP; ++n) {
+    h.h[n] = n < a.N && q.pos0 > 0 ? state[n] : 0.f;
+    h.A2[n] = n < a.N ? a.a[(size_t)c * a.N + n] * 1.4426950408889634f : 0.f;
+  }
+  const float D = a.d != nullptr ? a.d[c] : 0.f, bias = a.dt_bias != nullptr ? a.dt_bias[c] : 0.f;
+#pragma unroll 1
+  for (int r = q.t0; r < q.t1; ++r) {
+    const float u = ssm_load(a.u, r, c), s = ssm_softplus(ssm_load(a.dt, r, c) + bias);
+    float e[NP], bv[NP], cv[NP];
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+      bv[n] = n < a.N ? ssm_load(a.b, r, n) : 0.f;
+      cv[n] = n < a.N ? ssm_load(a.c, r, n) : 0.f;
+    }
+    h.decays(s, e);
+    h.token(e, __fmul_rn(s, u), bv, cv);
+    float v = fmaf(D, u, h.without_rest(cv, 0, a.N));
+    if (a.z.p != nullptr) v = __fmul_rn(v, ssm_silu(ssm_load(a.z, r, c)));
+    ssm_store(a.y, r, c, v);
+  }
+#pragma unroll
+  for (int n = 0; n < NP; ++n)
+    if (n < a.N) state[n] = h.h[n];
+}
+template <int NP, bool ALL, typename TU, typename TZ>
 __global__ void __launch_bounds__(ScanWide<NP>::CW) selective_scan_wide_kernel(const ScanArgs a) {
   using W = ScanWide<NP>;
   constexpr int CW = W::CW, SB = W::SB, TT = W::TT, STAGES = W::STAGES, PARTS = 2 * SB * NP / CW;
@@ -641,6 +705,10 @@ __global__ void __launch_bounds__(ScanWide<NP>::CW) selective_scan_wide_kernel(c
     if (i + 2 < blocks) keep_bc(i + 2);
   }
   pdl_launch_dependents();
+  if (!ALL && h.h[NP - 1] != 0.f) {  // (NaN)
+    if (c < a.C) scan_channel<NP>(a, q, c);
+    return;
+  }
   if (c < a.C)
 #pragma unroll
     for (int n = 0; n < NP; ++n)
@@ -650,7 +718,7 @@ __global__ void __launch_bounds__(ScanWide<NP>::CW) selective_scan_wide_kernel(c
 // Steps of one row per sequence.  grid (channels / (128 / L), B / L): a thread takes its states of L sequences through their tokens,
 // lane l prepares and ends one sequence's.  Bound by memory: the states are read and written once (256 sequences of 5120 channels with
 // 16 states: 40.6 us, 4.5 TB/s; with nine blocks to an SM 43, with a group's loads ahead of the one before it, which takes registers, 49).
-template <int L, int S>
+template <int L, int S, bool ALL>
 __global__ void __launch_bounds__(128, L * S <= 16 ? 10 : 1) selective_step_kernel(const ScanArgs a) {
   pdl_launch_dependents();
   pdl_wait();
@@ -718,6 +786,8 @@ __global__ void __launch_bounds__(128, L * S <= 16 ? 10 : 1) selective_step_kern
     float e[S];
     h.decays(dtj, e);
     acc[j] = h.token(e, duj, bv, cv);
+    if constexpr (!ALL)
+      if (scan_strange(duj)) acc[j] = h.without_rest(cv, lane, a.N);
     if (c < a.C) {
       float* to = a.state + s * a.slot_stride + (size_t)cc * a.N;
       if (S >= 4 && a.whole) {

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oxidize_b200 import ops
-from test_state_space import DEVICES, scan_inputs, step
+from test_state_space import DEVICES, scan64, scan_inputs, step
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -108,3 +108,49 @@ def test_models_with_many_states(states, tmp_path):
         a, b = cpu.next_token_logits(prompts), gpu.next_token_logits(prompts)
         assert _far(b, a) < 0.1
         prompts = [p + [int(torch.as_tensor(a)[i].argmax())] for i, p in enumerate(prompts)]
+
+
+# lens, channels: single rows; 16 and 8 lanes and one lane to a channel (with 148 SMs, see lanes())
+STEPS = {"single rows": ([1] * 9, 40), "16 lanes": ([70, 3, 17], 40), "8 lanes": ([37, 70], 1801), "one lane": ([70, 70, 70, 64, 33, 70, 1, 70], 2726)}
+
+
+def lanes(lens, C):
+    """Lanes to a channel of up to 16 states that the device's kernel takes, of its rule on the channels that run at a time."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    channels = C * -(-sum(lens) // max(lens))
+    return 16 if channels < 12 * sms else 8 if channels < 110 * sms else 1
+
+
+def check_kernel(kind, lens, C):
+    if torch.cuda.get_device_properties(0).multi_processor_count == 148:
+        assert kind == "single rows" or lanes(lens, C) == {"16 lanes": 16, "8 lanes": 8, "one lane": 1}[kind]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("kind", list(STEPS))
+@pytest.mark.parametrize("N,gate,types", [(1, False, "f32"), (5, True, "f32"), (8, False, "bf16"), (11, False, "f32"), (13, True, "bf16"), (16, True, "f32"), (24, False, "f32"),
+                                          (100, True, "f32")])
+def test_steps_that_are_not_finite(N, gate, types, kind, device):
+    """Inputs and steps that are infinite or NaN: infinities stay infinities, whatever the number of states is padded to."""
+    lens, C = STEPS[kind]
+    if device == "cpu" and C > 100:
+        pytest.skip("the CPU has one statement for all of them")
+    if device == "cuda":
+        check_kernel(kind, lens, C)
+    gen = torch.Generator().manual_seed(51)
+    meta = step(lens, device, slots=range(len(lens)))
+    v = scan_inputs(gen, sum(lens), C, N, types, types, "f32", "f32", gate, True, True, 0, device)
+    v["b"], v["c"] = v["b"].abs(), v["c"].abs()  # (sums of infinities of one sign)
+    end = int(meta.query_start[1])
+    strange = {(end - 1, 3): ("u", float("inf")), (0, 7): ("u", float("-inf")), (end // 2, C - 1): ("dt", float("inf")), (end, 5): ("u", float("nan")),
+               (sum(lens) - 1, 0): ("u", float("inf"))}
+    for (t, c), (name, value) in strange.items():
+        v[name][t, c] = value
+    state = torch.randn(len(lens) + 2, C, N, generator=gen).to(device)
+    want, err, after, after_err = scan64(**v, meta=meta, state=state)
+    y = ops.selective_scan(**v, meta=meta, state=state)
+    assert torch.isinf(want).any() and torch.isnan(want).any()
+    for got, exact, bound in ((y.double(), want, err), (state.double(), after, after_err)):
+        fine = torch.isfinite(exact)
+        assert ((got - exact).abs() <= bound)[fine].all()
+        assert torch.equal(torch.isnan(got), torch.isnan(exact)) and torch.equal(got[torch.isinf(exact)], exact[torch.isinf(exact)])
