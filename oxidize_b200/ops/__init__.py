@@ -241,7 +241,7 @@ def causal_conv(x, w, bias, meta, window, act="silu", act_dtype=torch.float32, o
     row is row p % taps) and is updated; ``meta`` gives query_start, seq_lens, state_slots (no slot twice) and max_query_len.  Nothing
     comes before position 0; rows of a sequence without a slot become zeros, rows behind the last sequence are left as they are.  A slot
     past the store, or a length below the sequence's rows, is an error on the CPU; the device takes it for no slot and reports it in
-    its status word."""
+    its status word.  ``out`` may lie over an input, which is copied then."""
     _check_recurrent(meta, window, "window")
     T, C = x.shape
     taps = w.shape[1]

@@ -87,13 +87,34 @@ def _out(out: Optional[torch.Tensor], T: int, C: int, dtype: torch.dtype, like: 
     return out
 
 
+def _extent(v: torch.Tensor):
+    """First byte of a matrix, bytes of it whole and of a row."""
+    (T, C), (ld, one), size = v.shape, v.stride(), v.element_size()
+    row = ((C - 1) * one + 1) * size
+    return v.data_ptr(), (T - 1) * ld * size + row, row
+
+
+def _apart(v: Optional[torch.Tensor], out: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """v, or a copy of it where ``out`` shares memory with it: rows are read after others were written.  Columns side by side in rows of
+    one length share none."""
+    if v is None or out is None or out.dim() != 2 or v.numel() == 0 or out.numel() == 0:
+        return v
+    (at, size, row), (at_out, size_out, row_out) = _extent(v), _extent(out)
+    if at + size <= at_out or at_out + size_out <= at:
+        return v
+    ld = v.stride(0) * v.element_size()
+    if v.shape[0] > 1 and ld == out.stride(0) * out.element_size() and row <= (at_out - at) % ld <= ld - row_out:
+        return v
+    return v.clone()
+
+
 def causal_conv(x, w, bias, meta, window, act, act_dtype, out=None):
     T, C = x.shape
     here = torch._C._cuda_getDevice()
     if not (x.get_device() == w.get_device() == window.get_device() == here and (bias is None or bias.get_device() == here)
             and (out is None or out.get_device() == here)):
         raise _elsewhere(here, x=x, w=w, bias=bias, window=window, out=out)
-    x, at_x = _rows(x, "x")
+    x, at_x = _rows(_apart(x, out), "x")
     w, bias = _floats(w, "w"), _floats(bias, "bias")
     seqs, B = _sequences(meta, here)
     y = _out(out, T, C, act_dtype, x)
@@ -114,6 +135,8 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype, out=No
         raise _elsewhere(here, u=u, dt=dt, a=a, b=b, c=c, d=d, z=z, dt_bias=dt_bias, state=state, out=out)
     if u.dtype != dt.dtype and u.dtype in DT and dt.dtype in DT:  # (the kernels read them as one type)
         u, dt = u.float(), dt.float()
+    if out is not None:
+        u, dt, b, c, z = (_apart(v, out) for v in (u, dt, b, c, z))
     (u, at_u), (dt, at_dt), (b, at_b), (c, at_c) = _rows(u, "u"), _rows(dt, "dt"), _rows(b, "b"), _rows(c, "c")
     z, at_z = (None, (None, 0, 0)) if z is None else _rows(z, "z")
     a, d, dt_bias = _floats(a, "a"), _floats(d, "d"), _floats(dt_bias, "dt_bias")

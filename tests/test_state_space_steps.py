@@ -154,3 +154,59 @@ def test_steps_that_are_not_finite(N, gate, types, kind, device):
         fine = torch.isfinite(exact)
         assert ((got - exact).abs() <= bound)[fine].all()
         assert torch.equal(torch.isnan(got), torch.isnan(exact)) and torch.equal(got[torch.isinf(exact)], exact[torch.isinf(exact)])
+
+
+def test_what_shares_memory_with_an_output():
+    """Against the sets of bytes themselves."""
+    from oxidize_b200.ops import cuda_ssm
+
+    store = torch.zeros(400)
+    gen = torch.Generator().manual_seed(61)
+    pick = lambda n: int(torch.randint(0, n, (1,), generator=gen))  # noqa: E731
+
+    def matrix(ld):
+        v = store if pick(3) else store.view(torch.bfloat16)
+        return v.as_strided((T, 1 + pick(9)), (ld * (4 // v.element_size()), 1), pick(90))
+
+    def held(v):
+        rows = range(v.shape[0])
+        return {v.data_ptr() + (r * v.stride(0) + c) * v.element_size() + b for r in rows for c in range(v.shape[1]) for b in range(v.element_size())}
+
+    seen = set()
+    for _ in range(2000):
+        T = 1 + pick(5)
+        ld = 9 + pick(12)
+        v, out = matrix(ld), matrix(ld if pick(4) else 9 + pick(12))
+        shared = bool(held(v) & held(out))
+        copied = cuda_ssm._apart(v, out).data_ptr() != v.data_ptr()
+        # rows of other lengths count as sharing as soon as the matrices interleave
+        assert copied == shared if v.stride(0) * v.element_size() == out.stride(0) * out.element_size() else copied >= shared
+        seen.add((shared, copied))
+    assert {(True, True), (False, False)} <= seen
+    assert cuda_ssm._apart(None, store[None]) is None and cuda_ssm._apart(store[None], None) is not None
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens", [[1] * 6, [300, 1, 64]])
+def test_outputs_over_inputs(lens, device):
+    """Over the input itself, or one row further: as into memory of its own."""
+    gen = torch.Generator().manual_seed(62)
+    C, N, T = 72, 11, sum(lens)
+    meta = step(lens, device)
+    w = torch.randn(C, 4, generator=gen).to(device)
+    v = scan_inputs(gen, T, C, N, "f32", "f32", "f32", "f32", True, True, True, 0, device)
+    v["u"][T // 2, 3] = float("inf")
+    window, state = torch.randn(len(lens) + 2, 4, C, generator=gen).to(device), torch.randn(len(lens) + 2, C, N, generator=gen).to(device)
+    conv = lambda x, out: ops.causal_conv(x, w, None, meta, window.clone(), out=out)  # noqa: E731
+    scan = lambda name, x, out: ops.selective_scan(**dict(v, **{name: x}), meta=meta, state=state.clone(), out=out)  # noqa: E731
+    same = lambda a, b: torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))  # noqa: E731
+    for name, call in [("u", lambda x, out: conv(x, out))] + [(n, lambda x, out, n=n: scan(n, x, out)) for n in ("u", "dt", "z")]:
+        # over it, a row further, and columns beside it (the same strides either way: the CPU takes vector and scalar forms of its functions
+        # by them)
+        for ahead, beside in ((0, 0), (C, 0), (0, C)):
+            room = torch.zeros((T + 1) * (C + beside), device=device)
+            x, out = (room.as_strided((T, C), (C + beside, 1), at) for at in (0, ahead + beside))
+            x.copy_(v[name])
+            want = call(x, None)
+            got = call(x, out)
+            assert got is out and same(got, want)
