@@ -66,7 +66,7 @@ static int scan_lanes(int C, int T, int longest) {
 
 // Selective scan of a step: u, dt, z, y of C channels and b, c of N <= 128 states, each a matrix of T rows with its own stride and
 // dtype (u and dt: the same one); a [C, N]; d, dt_bias [C] or null; z null: no gate.  The state [num_slots, C, N] float32 is read and updated.
-// longest 1: every sequence feeds one row at most.
+// longest 1: every sequence feeds one row at most (one with more is reported: its rows become zeros, its state stays).
 OXB_API int oxb_selective_scan(const void* u, int ld_u, int u_dtype, const void* dt, int ld_dt, int dt_dtype, const void* z, int ld_z,
                                int z_dtype, const void* b, int ld_b, int b_dtype, const void* c, int ld_c, int c_dtype, const float* a,
                                const float* d, const float* dt_bias, const int* query_start, const int* seq_lens, const int* slots,

@@ -727,6 +727,11 @@ __global__ void __launch_bounds__(128, L * S <= 16 ? 10 : 1) selective_step_kern
   SsmSeq q{0, 0, -1, 0};
   if (b < a.s.B) q = ssm_seq(a.s, b, blockIdx.x == 0 && threadIdx.x < L);
   const bool on = q.t1 == q.t0 + 1, live = on && q.slot >= 0;
+  if (q.t1 > q.t0 + 1) {  // more rows than the caller said
+    if (blockIdx.x == 0 && threadIdx.x < L) oxb_report(OXB_BAD_ARGUMENT, q.t1 - q.t0);
+    if (c < a.C)
+      for (int t = q.t0; t < q.t1; ++t) ssm_store(a.y, t, c, 0.f);
+  }
   uint32_t ub = 0, db = 0, zb = 0;
   if (live) {
     ub = ssm_bits(a.u, q.t0, cc);

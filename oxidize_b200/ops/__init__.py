@@ -261,7 +261,8 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype=torch.f
     """Selective state-space recurrence over a step's rows, each sequence from its own state: s = softplus(dt + dt_bias);
     h <- exp(s a) h + s u b; y = (h . c + d u) silu(z) in ``act_dtype``.  u, dt, z [T, C] and b, c [T, N] (bfloat16 or float32, possibly
     columns of wider projections; z None: no gate); a [C, N], d [C], dt_bias [C] float32 (d, dt_bias None: zeros); ``state`` [slots, C,
-    N] float32 is updated.  ``meta`` as for ``causal_conv``.  A sequence whose rows start at position 0 starts from nothing; rows of
+    N] float32 is updated.  ``meta`` as for ``causal_conv``; a sequence with more than
+    one row where max_query_len is 1 becomes rows of zeros on the device, which reports it in its status word.  A sequence whose rows start at position 0 starts from nothing; rows of
     one without a slot become zeros, rows behind the last sequence are left as they are.  A sequence's result does not depend on
     the portions that its rows come in, nor on its neighbours.  On the device N is at most ``MAX_SCAN_STATES``."""
     _check_recurrent(meta, state, "state")

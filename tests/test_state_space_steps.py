@@ -210,3 +210,26 @@ def test_outputs_over_inputs(lens, device):
             want = call(x, None)
             got = call(x, out)
             assert got is out and same(got, want)
+
+
+@pytest.mark.gpu
+def test_more_rows_than_the_step_says():
+    """max_query_len 1 (which metadata has where nobody sets it) and a sequence of three rows: reported, zeros, its state as it was; the
+    others as ever.  The convolution does not go by it."""
+    from oxidize_b200.ops import cuda as K
+
+    gen = torch.Generator().manual_seed(71)
+    C, N, lens = 200, 16, [1, 3, 1, 0, 1]
+    meta = step(lens, "cuda", slots=(0, 1, 2, 3, 4), fresh=())
+    v = scan_inputs(gen, 6, C, N, "f32", "f32", "f32", "f32", True, True, True, 0, "cuda")
+    w, window, state = torch.randn(C, 4, generator=gen).cuda(), torch.randn(7, 4, C, generator=gen).cuda(), torch.randn(7, C, N, generator=gen).cuda()
+    window1, state1 = window.clone(), state.clone()
+    y, s = ops.causal_conv(v["u"], w, None, meta, window), ops.selective_scan(**v, meta=meta, state=state)
+    kept = state1.clone()
+    meta.max_query_len = 1
+    K.status()
+    assert torch.equal(ops.causal_conv(v["u"], w, None, meta, window1), y) and torch.equal(window, window1) and K.status()[0] == 0
+    s1 = ops.selective_scan(**v, meta=meta, state=state1, out=torch.full_like(s, 7.0))
+    assert K.status()[:2] == (8, 3)
+    assert (s1[1:4] == 0).all() and torch.equal(s1[[0, 4, 5]], s[[0, 4, 5]])
+    assert torch.equal(state1[1], kept[1]) and torch.equal(state1[[0, 2, 3, 4, 5, 6]], state[[0, 2, 3, 4, 5, 6]])
