@@ -90,3 +90,18 @@ def test_large_tokens(T, device):
     y = ops.linear(x, LinearWeight([q]))
     assert torch.isfinite(y).all() and y.abs().max() > 1e35
     check(x, q, None, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 2, 40, 300])
+@pytest.mark.parametrize("k", [40959, 1023, 500, 17, 130])
+def test_nothing_is_read_behind_a_row(k, T):
+    """Codes between which, and behind the last of which, other codes lie in the same memory: none of them counts."""
+    gen = torch.Generator().manual_seed(k)
+    n, ld = 70, (k + 15) // 16 * 16
+    room = torch.full((n * ld + 512,), 127, dtype=torch.int8, device="cuda")
+    codes = room.as_strided((n, k), (ld, 1))
+    codes.copy_(torch.randint(-127, 128, (n, k), generator=gen).to(torch.int8))
+    q = QTensor("I8", codes, (n, k), (torch.rand(n, generator=gen) * 0.01).cuda())
+    x = torch.randn(T, k, generator=gen).bfloat16().cuda()
+    check(x, q, None, ops.linear(x, LinearWeight([q])))

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from oxidize_b200 import ops
-from test_state_space import DEVICES, scan64, scan_inputs, step
+from test_state_space import DEVICES, TYPE, out_bound, scan64, scan_inputs, step
 
 
 @pytest.mark.parametrize("device", DEVICES)
@@ -233,3 +233,68 @@ def test_more_rows_than_the_step_says():
     assert K.status()[:2] == (8, 3)
     assert (s1[1:4] == 0).all() and torch.equal(s1[[0, 4, 5]], s[[0, 4, 5]])
     assert torch.equal(state1[1], kept[1]) and torch.equal(state1[[0, 2, 3, 4, 5, 6]], state[[0, 2, 3, 4, 5, 6]])
+
+
+# Lengths off the tiles' multiples (8 and 32 rows), with none and with one row; channels off 32
+WIDE = [70, 64, 0, 33, 70, 1, 61, 70, 70, 58, 9]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,C,tu,tbc,tout,gate", [(16, 2726, "f32", "f32", "bf16", True), (16, 2726, "bf16", "bf16", "f32", True), (16, 5121, "bf16", "f32", "bf16", False),
+                                                  (11, 2726, "f32", "bf16", "f32", True), (12, 2752, "bf16", "f32", "f32", False), (8, 2726, "f32", "f32", "f32", True),
+                                                  (5, 2735, "bf16", "bf16", "bf16", False), (8, 2752, "bf16", "bf16", "f32", False), (3, 2726, "f32", "f32", "bf16", True)])
+def test_scan_with_a_lane_to_a_channel(N, C, tu, tbc, tout, gate):
+    """Wide steps of prompts, one of which has no slot and one no rows."""
+    gen = torch.Generator().manual_seed(81)
+    check_kernel("one lane", WIDE, C)
+    meta = step(WIDE, "cuda", no_slot=(4,))
+    T = sum(WIDE)
+    v = scan_inputs(gen, T + 2, C, N, tu, tu, tbc, tout, gate, True, True, 5, "cuda")
+    state = torch.randn(len(WIDE) + 2, C, N, generator=gen).cuda()
+    want, err, after, after_err = scan64(**v, meta=meta, state=state)
+    out = torch.full((T + 2, C + 3), 7.0, dtype=TYPE[tout], device="cuda")
+    y = ops.selective_scan(**v, meta=meta, state=state, act_dtype=TYPE[tout], out=out[:, 2 : 2 + C])[:T]
+    assert ((y.double() - want[:T]).abs() <= out_bound(want, err, TYPE[tout])[:T]).all()
+    assert ((state.double() - after).abs() <= after_err).all()
+    assert (out[T:] == 7).all() and (out[:, :2] == 7).all() and (out[:, 2 + C :] == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,C", [(24, 1777), (32, 2001), (20, 6003)])
+def test_scan_of_more_states_on_eight_lanes(N, C):
+    gen = torch.Generator().manual_seed(82)
+    lens = [70, 37, 1, 70]
+    assert torch.cuda.get_device_properties(0).multi_processor_count != 148 or lanes(lens, C) <= 8
+    meta = step(lens, "cuda")
+    v = scan_inputs(gen, sum(lens), C, N, "f32", "f32", "f32", "f32", True, True, True, 3, "cuda")
+    state = torch.randn(len(lens) + 2, C, N, generator=gen).cuda()
+    want, err, after, after_err = scan64(**v, meta=meta, state=state)
+    y = ops.selective_scan(**v, meta=meta, state=state)
+    assert ((y.double() - want).abs() <= err).all() and ((state.double() - after).abs() <= after_err).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N", [16, 11, 8, 24])
+def test_neighbours_that_change_the_kernel_leave_the_bits(N):
+    """A sequence alone (8 lanes to a channel), in single rows, and beside others that bring a lane to a channel."""
+    gen = torch.Generator().manual_seed(83)
+    C, n = 2726, 70
+    check_kernel("one lane", WIDE, C)
+    check_kernel("8 lanes", [n], C)
+    v = scan_inputs(gen, sum(WIDE), C, N, "f32", "f32", "f32", "f32", True, True, True, 0, "cuda")
+    first = torch.randn(1, C, N, generator=gen).cuda()
+    take = lambda rows: {k: m[rows] if k in ("u", "dt", "b", "c", "z") else m for k, m in v.items()}  # noqa: E731
+    many = torch.randn(len(WIDE), C, N, generator=gen).cuda()
+    many[0] = first[0]
+    alone, rows = first.clone(), first.clone()
+
+    def meta(lens, before, slots):
+        m = step(lens, "cuda", slots=slots)
+        m.seq_lens.copy_(torch.tensor([before + k for k in lens]))
+        return m
+
+    y = ops.selective_scan(**v, meta=meta(WIDE, 6, range(len(WIDE))), state=many)[:n]
+    assert torch.equal(ops.selective_scan(**take(slice(0, n)), meta=meta([n], 6, (0,)), state=alone), y) and torch.equal(alone[0], many[0])
+    for t in range(n):
+        assert torch.equal(ops.selective_scan(**take(slice(t, t + 1)), meta=meta([1], 6 + t, (0,)), state=rows), y[t : t + 1])
+    assert torch.equal(rows[0], many[0])
