@@ -242,7 +242,7 @@ def causal_conv(x, w, bias, meta, window, act="silu", act_dtype=torch.float32, o
     comes before position 0; rows of a sequence without a slot become zeros, rows behind the last sequence are left as they are.  A slot
     past the store, or a length below the sequence's rows, is an error on the CPU; the device takes it for no slot and reports it in
     its status word.  ``out`` may lie over an input, which is copied then."""
-    _check_recurrent(meta, window, "window")
+    _check_recurrent(meta, window, "window", out)
     T, C = x.shape
     taps = w.shape[1]
     if w.shape[0] != C or taps < 1 or window.shape[1:] != (taps, C) or (bias is not None and bias.shape != (C,)):
@@ -265,7 +265,7 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype=torch.f
     one row where max_query_len is 1 becomes rows of zeros on the device, which reports it in its status word.  A sequence whose rows start at position 0 starts from nothing; rows of
     one without a slot become zeros, rows behind the last sequence are left as they are.  A sequence's result does not depend on
     the portions that its rows come in, nor on its neighbours.  On the device N is at most ``MAX_SCAN_STATES``."""
-    _check_recurrent(meta, state, "state")
+    _check_recurrent(meta, state, "state", out)
     T, C = u.shape
     N = a.shape[1]
     if (dt.shape != (T, C) or a.shape != (C, N) or b.shape != (T, N) or c.shape != (T, N) or state.shape[1:] != (C, N)
@@ -278,11 +278,13 @@ def selective_scan(u, dt, a, b, c, d, z, dt_bias, meta, state, act_dtype=torch.f
     return y if out is None else _into(out, y, meta)
 
 
-def _check_recurrent(meta, kept, what):
+def _check_recurrent(meta, kept, what, out):
     if meta.state_slots is None:
         raise ValueError("a layer with a recurrent state needs the sequences' state slots")
     if kept.dtype != torch.float32 or kept.dim() != 3:
         raise ValueError(f"{what} is float32 with three dimensions, not {kept.dtype} {tuple(kept.shape)}")
+    if out is not None and out.dim() == 2 and out.shape[0] > 1 and out.stride(1) <= 1 and out.stride(0) < out.shape[1]:
+        raise ValueError(f"rows of out share memory: strides are {out.stride()}")
 
 
 def _into(out, y, meta):

@@ -103,7 +103,7 @@ def _apart(v: Optional[torch.Tensor], out: Optional[torch.Tensor]) -> Optional[t
     if at + size <= at_out or at_out + size_out <= at:
         return v
     ld = v.stride(0) * v.element_size()
-    if v.shape[0] > 1 and ld == out.stride(0) * out.element_size() and row <= (at_out - at) % ld <= ld - row_out:
+    if v.shape[0] > 1 and ld > 0 and ld == out.stride(0) * out.element_size() and row <= (at_out - at) % ld <= ld - row_out:
         return v
     return v.clone()
 

@@ -298,3 +298,23 @@ def test_neighbours_that_change_the_kernel_leave_the_bits(N):
     for t in range(n):
         assert torch.equal(ops.selective_scan(**take(slice(t, t + 1)), meta=meta([1], 6 + t, (0,)), state=rows), y[t : t + 1])
     assert torch.equal(rows[0], many[0])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("lens", [[1, 1, 1], [3]])
+def test_outputs_whose_rows_share_memory_are_refused(lens, device):
+    """Also over an input of that kind; a row alone shares with no other."""
+    gen = torch.Generator().manual_seed(91)
+    C, meta = 8, step(lens, device)
+    w, window, state = torch.zeros(C, 4, device=device), torch.zeros(5, 4, C, device=device), torch.zeros(5, C, 16, device=device)
+    v = scan_inputs(gen, 3, C, 16, "f32", "f32", "f32", "f32", True, True, True, 0, device)
+    room = torch.zeros(64, device=device)
+    for apart in (0, 7):
+        out = room.as_strided((3, C), (apart, 1))
+        for x in (v["u"], out):
+            with pytest.raises(ValueError, match="share"):
+                ops.causal_conv(x, w, None, meta, window, out=out)
+            with pytest.raises(ValueError, match="share"):
+                ops.selective_scan(**dict(v, u=x), meta=meta, state=state, out=out)
+    one = step([1], device)
+    ops.causal_conv(v["u"][:1], w, None, one, window, out=room.as_strided((1, C), (0, 1)))
