@@ -220,9 +220,11 @@ __device__ __forceinline__ void umma_i8(uint32_t tmem_d, uint64_t adesc, uint64_
 constexpr int I8_BM = 128, I8_BK = 128;  // weight rows of an MMA; values of a k-block (one 128-byte swizzle row)
 constexpr int I8_THREADS = 192;          // warps 0-3: epilogue, 4: TMA, 5: MMA (which owns the tensor memory)
 
-// A tile of 128 RB weight rows x TN tokens.  What comes from L2 to all SMs bounds many tokens (128 x 256: 48 KB per 512 clocks of products on
-// every SM, 27 TB/s; some 11 come), so those take tiles of 256 x 256, which fill the tensor memory with their two accumulators: a
-// third less per product (8192 tokens of 8192 x 8192: 445 to 474 us, 2.3 to 2.5 P operations a second; 575 with 128 x 256).
+// A tile of 128 RB weight rows x TN tokens.  A tile of 128 x 256 wants 48 KB per 512 clocks of products on every SM (27 TB/s over all of them),
+// so many tokens take tiles of 256 x 256, which fill the tensor memory with their two accumulators: a third less per product (8192
+// tokens of 8192 x 8192: 445 to 474 us, 2.3 to 2.5 P operations a second; 575 with 128 x 256).  Which limit those meet is not established:
+// 64 bytes a clock come into each SM (some 11 TB/s over all of them at the measured time), and shared memory takes those and gives the
+// products 96 more, with 128 a clock.
 template <int TN, int RB>
 struct I8Tile {
   static constexpr int A_BYTES = RB * I8_BM * I8_BK, B_BYTES = TN * I8_BK, STAGE_BYTES = A_BYTES + B_BYTES;
@@ -260,8 +262,9 @@ __device__ __forceinline__ void int8_store_rows(const __nv_bfloat16* stage, int 
   }
 }
 
-// grid (tiles, splits).  RB = 2: the tiles of a last wave that fills less than half of the SMs come as halves.  With splits the CTAs of a tile are a cluster along K: whole-number sums meet in
-// distributed shared memory, each CTA ends its share of the tokens (in any order the same sum; RB = 1 only).
+// grid (tiles, splits).  RB = 2: the tiles of a last wave that fills less than half of the SMs come as halves.  With splits the CTAs of a
+// tile are a cluster along K: whole-number sums meet in distributed shared memory, each CTA ends its share of the tokens (in any order
+// the same sum; RB = 1 only).
 template <int TN, int RB>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 gemm_int8_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX, const I8Args a) {

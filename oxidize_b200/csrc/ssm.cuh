@@ -143,7 +143,8 @@ __device__ __forceinline__ float ssm_softplus(float x) {
 }
 
 // The y-th longest of a step's sequences: long ones start first, so that short ones fill the gaps (9 of 331 to 1650 rows, 5120
-// channels: 398 us, 501 in their own order).  More than 32 even out by themselves and stay in their order.  Whole warps.
+// channels: 398 us, 501 in their own order).  More than 32 stay in their order, also where a long one comes last: 200 single rows ahead of
+// a portion of 2048 take 668 us, where the portion alone takes 193.  Whole warps.
 __device__ __forceinline__ int scan_sequence(const SsmStep& s, int y) {
   if (s.B > 32) return y;
   const int lane = threadIdx.x & 31, n = lane < s.B ? s.query_start[lane + 1] - s.query_start[lane] : -1;
@@ -322,8 +323,8 @@ struct ScanTile {
 // registers (as they are stored: a conversion would wait for its load) a tile ahead of their use, makes its tokens' steps, hands them
 // to the other lanes of the channel, and ends the tokens whose sums it gets.
 //
-// Alone on its quarter of an SM a warp takes as long as its instructions' latencies: 58 ns a token of 16 states with L = 8, 30 with 16
-// (2048 rows of 1536 channels 104 us, of 256 channels 62).  With more warps it is bound by what shared memory can put into registers, 32
+// Alone on its quarter of an SM a warp takes as long as its instructions' latencies (the recurrence itself is one fused multiply-add a
+// token): 58 ns a token of 16 states with L = 8, 30 with 16 (2048 rows of 1536 channels 101 us, of 256 channels 62).  With more warps it is bound by what shared memory can put into registers, 32
 // values a clock and SM: the step and b and c for every lane of every channel, some 3 clocks per token and channel, against 1.2 for the
 // 19 special functions (16 decays, the step's, two for the gate).
 //
@@ -543,7 +544,8 @@ __global__ void __launch_bounds__(128) selective_scan_kernel(const ScanArgs a) {
 //
 // Bound by its instructions: 174 of them for a token and warp, which fill 64 % of the issue slots, and 20 special functions a channel (the
 // 16 decays among them), 56 % of that unit's; 248 registers leave two warps to a scheduler (with 168, three, 404 us).  9 sequences
-// of 331 to 1650 rows, 5120 channels: 398 us where the special functions alone take 189 and memory 60.
+// of 331 to 1650 rows, 5120 channels: 402 us where the special functions alone take 189 and memory 60.  Lengths that differ are part of it:
+// 1440 one-warp blocks on 1184 places, and the longest sequence runs to the end.
 template <int NP>
 struct ScanWide {
   static constexpr int CW = 32, SB = 32, TT = 8, STAGES = 3;
